@@ -283,6 +283,8 @@ def prepare(case, seed):
         for _, new in lengths:
             ctx.host_seq_start.append(ctx.host_seq_start[-1] + new)
         ctx.longest = max(new for _, new in lengths)
+        sequences = ctx.host_seq_slot, ctx.host_seq_start, ctx.host_seq_cached
+        ctx.seq_slot, ctx.seq_start, ctx.seq_cached = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in sequences)
         state["ctx"] = ctx
     return state
 
