@@ -133,6 +133,10 @@ class LayerMemory:
     state: Optional[torch.Tensor] = None  # [n_slots, *state_shape] float32
     tensor_maps: Optional[tuple] = None  # TMA descriptors of the group's (key, value) pools
     layer_index: int = 0  # this run's index within the group's pools
+    #: a cache in 8 bits: the scales of the pages' blocks, float32 [n_pages, Hkv], powers of two; the pages then hold e4m3
+    #: codes, keys as [n_pages, Hkv, page, hd], values as [n_pages, Hkv, page / 4, hd, 4] (four tokens' codes side by side)
+    k_scales: Optional[torch.Tensor] = None
+    v_scales: Optional[torch.Tensor] = None
 
 
 class StepMemories(list):

@@ -208,6 +208,17 @@ def attention_library(head_dim: int) -> ctypes.CDLL:
     )
 
 
+#: head sizes that the kernels of the cache in 8 bits are built for
+KV8_HEAD_DIMS = (64, 128, 256)
+
+
+def kv8_library(head_dim: int) -> ctypes.CDLL:
+    """The kernels of the paged cache in 8 bits, compiled per head size."""
+    if head_dim not in KV8_HEAD_DIMS:
+        raise ValueError(f"head size {head_dim} is not supported: the cache in 8 bits takes {KV8_HEAD_DIMS}")
+    return load(f"fg_kv8_hd{head_dim}", ["kv8.cu", "errors.cu"], [f"FG_HEAD_DIM={head_dim}"])
+
+
 def delta_rule_library() -> ctypes.CDLL:
     """The kernels of the gated delta rule (compiled when a model with such a mixer is bound)."""
     return load("fg_delta", ["delta_rule.cu", "errors.cu"])
@@ -247,5 +258,7 @@ def build_all(head_dims: Sequence[int] = (16, 32, 64, 128), latent_sizes: Sequen
     for rank, rot in latent_sizes:
         _compile(f"fg_latent_r{rank}_t{rot}", LATENT_SOURCES,
                  [f"FG_LATENT_RANK={rank}", f"FG_LATENT_ROT={rot}"])
+    for hd in KV8_HEAD_DIMS:
+        _compile(f"fg_kv8_hd{hd}", ["kv8.cu", "errors.cu"], [f"FG_HEAD_DIM={hd}"])
     for hd in head_dims:
         _compile(f"fg_attn_hd{hd}", ["attention.cu", "errors.cu"], [f"FG_HEAD_DIM={hd}"])

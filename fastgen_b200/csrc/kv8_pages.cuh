@@ -1,0 +1,466 @@
+// Writing and reading back the pages of the cache in 8 bits.
+#pragma once
+
+#include "kv8.cuh"
+
+namespace fg_kv8 {
+
+// ---------------------------------------------------------------------------------
+// The write.  A page's new tokens are a run: consecutive tokens of the step with the same request and page.  Its scale
+// needs the largest magnitude of the whole run (and the scale that the cached entries before it have), so a run is the
+// work of one block, found on the device: a block looks at STRETCH tokens, one a warp, and takes the runs that begin among
+// them, for one key/value head and keys or values.  A run of one token (a decoded token) is its warp's work; a longer run
+// is the block's, a warp for four slots at a time.  Blocks of the same stretch with higher indices rotate the queries.
+// ---------------------------------------------------------------------------------
+constexpr int STRETCH = 16;
+constexpr int WRITE_THREADS = 32 * STRETCH;
+constexpr int Q_SLICE = 8;  // query heads a block rotates
+
+// A lane's E = HD / 32 neighbouring elements of a row.
+template <int E, bool VEC>
+__device__ __forceinline__ void load_lane(float (&x)[E], const __nv_bfloat16* row, int lane) {
+  const __nv_bfloat16* p = row + lane * E;
+  uint32_t w[E / 2];
+  if constexpr (VEC) {
+    if constexpr (E == 2) {
+      w[0] = ld_global_4(p);
+    } else if constexpr (E == 4) {
+      asm volatile("ld.global.v2.u32 {%0,%1}, [%2];\n" : "=r"(w[0]), "=r"(w[1]) : "l"(p) : "memory");
+    } else {
+      const uint4 v = ld_global_16(p);
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    }
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  } else {
+    const volatile unsigned short* s = reinterpret_cast<const volatile unsigned short*>(p);
+#pragma unroll
+    for (int i = 0; i < E; ++i) x[i] = __uint_as_float((uint32_t)s[i] << 16);
+  }
+}
+
+template <int HD, bool VEC>
+__global__ void __launch_bounds__(WRITE_THREADS)
+kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, const __nv_bfloat16* k, int k_stride,
+                 const __nv_bfloat16* v, int v_stride, const int* __restrict__ pos, const int* __restrict__ req,
+                 const float* __restrict__ freqs, const float* __restrict__ v_freqs, unsigned char* k_pages,
+                 unsigned char* v_pages, float* k_scales, float* v_scales, const int* __restrict__ block_table, int table_width,
+                 int page_size, int n_pages, int n_tokens, int n_heads, int n_kv_heads, int* status, const float* rstd,
+                 const float* __restrict__ qn_w, const float* __restrict__ kn_w, int rstd_heads, float magnitude,
+                 int rot_pairs) {
+  constexpr int E = HD / 32;
+  __shared__ int s_len[STRETCH], s_page[STRETCH];
+  __shared__ float s_amax[STRETCH];
+  pdl_trigger();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int t0 = blockIdx.x * STRETCH, t = t0 + warp;
+  const int r = t < n_tokens ? req[t] : -1;
+  const int p = r >= 0 ? pos[t] : 0;
+  const int role = blockIdx.y;
+
+  // sine and cosine of the lane's pairs at position p
+  auto turns = [&](float (&sn)[E / 2], float (&cs)[E / 2], const float* table, int p, float mag) {
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+      sn[i] = 0.f;
+      cs[i] = 1.f;
+      if (table != nullptr) {
+        const int j = lane * (E / 2) + i;
+        sincosf((float)p * table[j], &sn[i], &cs[i]);
+        if (mag != 1.f && j < rot_pairs) {
+          sn[i] *= mag;
+          cs[i] *= mag;
+        }
+      }
+    }
+  };
+  auto turn = [&](float (&x)[E], const float (&sn)[E / 2], const float (&cs)[E / 2]) {
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+      const float a = x[2 * i], b = x[2 * i + 1];
+      x[2 * i] = a * cs[i] - b * sn[i];
+      x[2 * i + 1] = b * cs[i] + a * sn[i];
+    }
+  };
+  // the norm's factor of a token and head (column `at` of the factors, 0 or 1 where the whole projection shares one)
+  auto normed = [&](float (&x)[E], int t, int at_head, int at_whole, const float* w) {
+    if (rstd == nullptr) return;
+    const float f = rstd_heads ? rstd[(size_t)t * rstd_heads + at_head] : rstd[2 * (size_t)t + at_whole];
+#pragma unroll
+    for (int i = 0; i < E; ++i) x[i] *= f * (w ? w[lane * E + i] : 1.f);
+  };
+
+  if (role >= 2 * n_kv_heads) {
+    // ---- queries: a warp a token, the heads of the slice ----
+    if (r < 0) return;
+    float sn[E / 2], cs[E / 2];
+    turns(sn, cs, freqs, p, magnitude);
+    pdl_wait();
+    const int h0 = (role - 2 * n_kv_heads) * Q_SLICE, h1 = min(n_heads, h0 + Q_SLICE);
+    float x[Q_SLICE][E];
+#pragma unroll
+    for (int u = 0; u < Q_SLICE; ++u)
+      if (h0 + u < h1) load_lane<E, VEC>(x[u], q + (size_t)t * q_stride + (h0 + u) * HD, lane);
+#pragma unroll
+    for (int u = 0; u < Q_SLICE; ++u) {
+      const int h = h0 + u;
+      if (h >= h1) continue;
+      normed(x[u], t, h, 0, qn_w ? qn_w + h * HD : nullptr);
+      turn(x[u], sn, cs);
+      __nv_bfloat162 out[E / 2];
+#pragma unroll
+      for (int i = 0; i < E / 2; ++i) out[i] = __floats2bfloat162_rn(x[u][2 * i], x[u][2 * i + 1]);
+      __nv_bfloat16* dst = q_out + ((size_t)t * n_heads + h) * HD + lane * E;
+      if constexpr (VEC) {
+        if constexpr (E == 2) *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<uint32_t*>(out);
+        else if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(out);
+        else *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(out);
+      } else {
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i) dst[2 * i] = out[i].x, dst[2 * i + 1] = out[i].y;
+      }
+    }
+    return;
+  }
+
+  // ---- keys or values of one head ----
+  const int g = role >> 1;
+  const bool is_v = role & 1;
+  const __nv_bfloat16* src = (is_v ? v : k) + g * HD;
+  const int src_stride = is_v ? v_stride : k_stride;
+  unsigned char* pool = is_v ? v_pages : k_pages;
+  float* scales = is_v ? v_scales : k_scales;
+  const float* table = is_v ? v_freqs : freqs;
+  const float mag = is_v ? 1.f : magnitude;
+  const float* norm_w = kn_w ? kn_w + g * HD : nullptr;
+
+  // the run that begins at this warp's token: its length (0: none begins here) and its page
+  const int slot = p & (page_size - 1);
+  int len = 0, page = -1;
+  if (r >= 0 && (t == 0 || slot == 0 || req[t - 1] != r || pos[t - 1] != p - 1)) {
+    const int most = min(page_size - slot, n_tokens - t);
+    for (int at = 0; at < most; at += 32) {
+      const int i = at + lane;
+      const bool mine = i < most && req[t + i] == r && pos[t + i] == p + i;
+      const unsigned all = __ballot_sync(0xffffffffu, mine);
+      if (all != 0xffffffffu) {
+        len += __ffs(~all) - 1;
+        break;
+      }
+      len += 32;
+    }
+    const int logical = p / page_size;
+    page = logical < table_width ? block_table[(size_t)r * table_width + logical] : -1;
+    if (page < 0 || page >= n_pages) {
+      if (status && lane == 0) atomicOr(status, FG_STATUS_BAD_PAGE);
+      len = 0;
+    }
+  }
+  if (lane == 0) {
+    s_len[warp] = len;
+    s_page[warp] = page;
+  }
+  float sn[E / 2], cs[E / 2];
+  if (len == 1) turns(sn, cs, table, p, mag);
+  __syncthreads();
+  pdl_wait();
+
+  auto load_row = [&](float (&x)[E], int t) {
+    load_lane<E, VEC>(x, src + (size_t)t * src_stride, lane);
+    if (!is_v) normed(x, t, n_heads + g, 1, norm_w);
+  };
+  auto row_amax = [&](const float (&x)[E]) {
+    float a = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const float m = fabsf(x[i]);
+      if (m <= 3.402823466e38f) a = fmaxf(a, m);  // neither infinities nor NaNs
+    }
+    return a;
+  };
+  auto over = [&](float x, float f) { return fabsf(x) <= 3.402823466e38f ? x * f : __int_as_float(0x7fffffff); };
+  // the page's exponent: from the run's largest magnitude and, behind cached entries, no lower than theirs
+  auto exponents = [&](float amax, int slot, size_t block, int& old_e) {
+    int e = scale_exponent(amax);
+    old_e = e;
+    if (slot > 0) {
+      old_e = exponent_of_scale(__uint_as_float(ld_global_4(scales + block)));
+      e = max(e, old_e);
+    }
+    return e;
+  };
+  // cached entries before `slot` rounded again at a larger scale, by `n` threads of which this is number `i`
+  auto rescale = [&](size_t block, int slot, float f, int i, int n) {
+    unsigned char* base = pool + block * (size_t)page_size * HD;
+    const int whole = is_v ? (slot & ~3) * HD : slot * HD;  // bytes of whole rows (of whole groups of four rows)
+    for (int at = i * 4; at < whole; at += n * 4) {
+      uint32_t* w = reinterpret_cast<uint32_t*>(base + at);
+      *w = rescaled(ld_global_4(w), f);
+    }
+    if (is_v && (slot & 3)) {
+      const uint32_t mask = (1u << (8 * (slot & 3))) - 1u;  // tokens of the last group that are cached
+      for (int d = i; d < HD; d += n) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(base + whole) + d;
+        const uint32_t old = ld_global_4(w);
+        *w = (old & ~mask) | (rescaled(old, f) & mask);
+      }
+    }
+  };
+  // a lane's codes of one row
+  auto store_row = [&](const float (&x)[E], size_t block, int slot, float inv) {
+    unsigned char* base = pool + block * (size_t)page_size * HD;
+    uint32_t c[E / 2];
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) c[i] = codes_of(over(x[2 * i], inv), over(x[2 * i + 1], inv));
+    if (!is_v) {
+      unsigned char* dst = base + slot * HD + lane * E;
+      if constexpr (E == 2) *reinterpret_cast<uint16_t*>(dst) = (uint16_t)c[0];
+      else if constexpr (E == 4) *reinterpret_cast<uint32_t*>(dst) = c[0] | (c[1] << 16);
+      else *reinterpret_cast<uint2*>(dst) = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+    } else {
+      unsigned char* dst = base + (slot >> 2) * (4 * HD) + lane * (4 * E) + (slot & 3);
+#pragma unroll
+      for (int i = 0; i < E / 2; ++i) {
+        dst[8 * i] = (unsigned char)c[i];
+        dst[8 * i + 4] = (unsigned char)(c[i] >> 8);
+      }
+    }
+  };
+
+  if (len == 1) {
+    float x[E];
+    load_row(x, t);
+    turn(x, sn, cs);
+    const float amax = warp_max(row_amax(x));
+    const size_t block = (size_t)page * n_kv_heads + g;
+    int old_e;
+    const int e = exponents(amax, slot, block, old_e);
+    if (e > old_e) {
+      rescale(block, slot, exp2_int(max(old_e - e, -126)), lane, 32);
+      __syncwarp();
+    }
+    store_row(x, block, slot, exp2_int(-e));
+    __syncwarp();  // every lane has read the old scale
+    if (lane == 0 && (slot == 0 || e > old_e)) scales[block] = exp2_int(e);
+  }
+
+  for (int w = 0; w < STRETCH; ++w) {
+    const int n = s_len[w];
+    if (n <= 1) continue;
+    const int first = t0 + w, page = s_page[w];
+    const int p0 = pos[first], slot = p0 & (page_size - 1);
+    const size_t block = (size_t)page * n_kv_heads + g;
+    // four slots a warp and round; pages of up to 64 slots need one round, whose rows stay in registers
+    const int rounds = (page_size + 4 * STRETCH - 1) / (4 * STRETCH);
+    float x[4][E];
+    auto load_round = [&](int c) {
+      const int s0 = 4 * (warp + STRETCH * c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int s = s0 + i;
+#pragma unroll
+        for (int j = 0; j < E; ++j) x[i][j] = 0.f;
+        if (s >= slot && s < slot + n) load_row(x[i], first + s - slot);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int s = s0 + i;
+        if (table != nullptr && s >= slot && s < slot + n) {
+          float rs[E / 2], rc[E / 2];
+          turns(rs, rc, table, p0 + s - slot, mag);
+          turn(x[i], rs, rc);
+        }
+      }
+    };
+    float amax = 0.f;
+    for (int c = 0; c < rounds; ++c) {
+      load_round(c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) amax = fmaxf(amax, row_amax(x[i]));
+    }
+    amax = warp_max(amax);
+    __syncthreads();  // the run before is through with s_amax
+    if (lane == 0) s_amax[warp] = amax;
+    __syncthreads();
+    amax = warp_max(s_amax[lane & (STRETCH - 1)]);
+    int old_e;
+    const int e = exponents(amax, slot, block, old_e);
+    if (e > old_e) rescale(block, slot, exp2_int(max(old_e - e, -126)), threadIdx.x, WRITE_THREADS);
+    __syncthreads();  // rescaled entries share words with new ones; every thread has read the old scale
+    const float inv = exp2_int(-e);
+    for (int c = 0; c < rounds; ++c) {
+      if (rounds > 1) load_round(c);
+      const int s0 = 4 * (warp + STRETCH * c);
+      if (is_v && s0 >= slot && s0 + 4 <= slot + n) {
+        // a whole group of four tokens: words
+        uint32_t* dst = reinterpret_cast<uint32_t*>(pool + block * (size_t)page_size * HD + (size_t)s0 * HD) + lane * E;
+        uint32_t wd[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          wd[j] = codes_of(over(x[0][j], inv), over(x[1][j], inv)) | (codes_of(over(x[2][j], inv), over(x[3][j], inv)) << 16);
+        if constexpr (E == 2) {
+          *reinterpret_cast<uint2*>(dst) = make_uint2(wd[0], wd[1]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < E; j += 4) *reinterpret_cast<uint4*>(dst + j) = make_uint4(wd[j], wd[j + 1], wd[j + 2], wd[j + 3]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (s0 + i >= slot && s0 + i < slot + n) store_row(x[i], block, s0 + i, inv);
+      }
+    }
+    if (threadIdx.x == 0 && (slot == 0 || e > old_e)) scales[block] = exp2_int(e);
+  }
+}
+
+// ---------------------------------------------------------------------------------
+// What pages stand for, in bfloat16 [page, head, slot, HD]
+// ---------------------------------------------------------------------------------
+constexpr int EXPAND_THREADS = 256;
+
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// One (page, head) block: slots in [lo, hi) as what they stand for, the others as zeros.
+template <int HD>
+__device__ __forceinline__ void expand_block(const unsigned char* in, __nv_bfloat16* out, float scale, int page_size, bool is_v,
+                                             int lo, int hi) {
+  // a thread takes eight dimensions of four slots: four pieces of 16 bytes of the output
+  constexpr int PIECES = HD / 8;
+  for (int i = threadIdx.x; i < page_size / 4 * PIECES; i += EXPAND_THREADS) {
+    const int grp = i / PIECES, d = (i - grp * PIECES) * 8;
+    uint2 rows[4];  // eight codes of each slot
+    if (is_v) {
+      const uint4 a = ld_global_16(in + (size_t)grp * 4 * HD + d * 4), b = ld_global_16(in + (size_t)grp * 4 * HD + d * 4 + 16);
+      // word j holds dimension d + j of the four slots: a 4 x 4 transposition of bytes, twice
+      auto transpose = [](uint4 w, uint32_t (&o)[4]) {
+        const uint32_t x = __byte_perm(w.x, w.y, 0x5140), y = __byte_perm(w.z, w.w, 0x5140);
+        const uint32_t u = __byte_perm(w.x, w.y, 0x7362), v = __byte_perm(w.z, w.w, 0x7362);
+        o[0] = __byte_perm(x, y, 0x5410);
+        o[1] = __byte_perm(x, y, 0x7632);
+        o[2] = __byte_perm(u, v, 0x5410);
+        o[3] = __byte_perm(u, v, 0x7632);
+      };
+      uint32_t lo4[4], hi4[4];
+      transpose(a, lo4);
+      transpose(b, hi4);
+#pragma unroll
+      for (int s = 0; s < 4; ++s) rows[s] = make_uint2(lo4[s], hi4[s]);
+    } else {
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const unsigned char* src = in + (size_t)(grp * 4 + s) * HD + d;
+        asm volatile("ld.global.v2.u32 {%0,%1}, [%2];\n" : "=r"(rows[s].x), "=r"(rows[s].y) : "l"(src) : "memory");
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int slot = grp * 4 + s;
+      uint4 o = make_uint4(0, 0, 0, 0);
+      if (slot >= lo && slot < hi) {
+        const float2 a = floats_of(halves_of_low(rows[s].x)), b = floats_of(halves_of_high(rows[s].x));
+        const float2 c = floats_of(halves_of_low(rows[s].y)), e = floats_of(halves_of_high(rows[s].y));
+        o = make_uint4(bf16_pair(a.x * scale, a.y * scale), bf16_pair(b.x * scale, b.y * scale),
+                       bf16_pair(c.x * scale, c.y * scale), bf16_pair(e.x * scale, e.y * scale));
+      }
+      *reinterpret_cast<uint4*>(out + (size_t)slot * HD + d) = o;
+    }
+  }
+}
+
+template <int HD>
+__global__ void __launch_bounds__(EXPAND_THREADS)
+kv8_values_kernel(const unsigned char* k_pages, const unsigned char* v_pages, const float* k_scales, const float* v_scales,
+                  const int* pages, __nv_bfloat16* k_out, __nv_bfloat16* v_out, int page_size, int n_pages, int n_kv_heads,
+                  int* status) {
+  pdl_trigger();
+  pdl_wait();
+  const bool is_v = blockIdx.z == 1;
+  const int g = blockIdx.y, page = (int)ld_global_4(pages + blockIdx.x);
+  const size_t bytes = (size_t)page_size * HD;
+  __nv_bfloat16* out = (is_v ? v_out : k_out) + ((size_t)blockIdx.x * n_kv_heads + g) * bytes;
+  if (page < 0 || page >= n_pages) {
+    if (status && threadIdx.x == 0) atomicOr(status, FG_STATUS_BAD_PAGE);
+    for (size_t i = threadIdx.x; i < bytes / 8; i += EXPAND_THREADS) reinterpret_cast<uint4*>(out)[i] = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const size_t block = (size_t)page * n_kv_heads + g;
+  const float scale = __uint_as_float(ld_global_4((is_v ? v_scales : k_scales) + block));
+  expand_block<HD>((is_v ? v_pages : k_pages) + block * bytes, out, scale, page_size, is_v, 0, page_size);
+}
+
+// For prompt portions: blocks walk the (page, head) pairs that the sequences of two and more new tokens read.  Bound by
+// its bytes: a code in, two bytes out for each entry.
+template <int HD>
+__global__ void __launch_bounds__(EXPAND_THREADS)
+kv8_expand_kernel(const unsigned char* k_pages, const unsigned char* v_pages, const float* k_scales, const float* v_scales,
+                  const int* __restrict__ block_table, int table_width, const int* __restrict__ seq_slot,
+                  const int* __restrict__ seq_start, const int* __restrict__ seq_cached, int n_seqs, __nv_bfloat16* k_out,
+                  __nv_bfloat16* v_out, int page_size, int n_pages, int n_kv_heads, int window, int keep_first, int* status) {
+  __shared__ int s_slot[EXPAND_THREADS], s_cached[EXPAND_THREADS], s_last[EXPAND_THREADS], s_n;
+  pdl_trigger();
+  const int kept = (keep_first + page_size - 1) / page_size;
+  const size_t bytes = (size_t)page_size * HD;
+  const int grid = gridDim.x;
+  bool waited = false;
+  int before = 0;  // items of the sequences before, modulo the grid
+  for (int base = 0; base < n_seqs; base += EXPAND_THREADS) {
+    // the sequences of two and more tokens among the next EXPAND_THREADS, in any order of their own: every block must
+    // find the same one, so the first warp alone lists them
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      int n = 0;
+      for (int s0 = base; s0 < min(n_seqs, base + EXPAND_THREADS); s0 += 32) {
+        const int s = s0 + (int)threadIdx.x;
+        const int slot = s < n_seqs ? seq_slot[s] : -1;
+        const int fresh = slot >= 0 ? seq_start[s + 1] - seq_start[s] : 0;
+        const unsigned some = __ballot_sync(0xffffffffu, fresh >= 2);
+        if (fresh >= 2) {
+          const int at = n + __popc(some & ((1u << threadIdx.x) - 1u));
+          s_slot[at] = slot;
+          s_cached[at] = seq_cached[s];
+          s_last[at] = seq_cached[s] + fresh - 1;
+        }
+        n += __popc(some);
+      }
+      if (threadIdx.x == 0) s_n = n;
+    }
+    __syncthreads();
+    for (int s = 0; s < s_n; ++s) {
+      const int last = s_last[s];
+      const int lo_page = first_visible(s_cached[s], window) / page_size;
+      const int n_kept = min(kept, lo_page);
+      const int items = (n_kept + last / page_size - lo_page + 1) * n_kv_heads * 2;
+      // the blocks take the items of all sequences in turn
+      const int first = ((int)blockIdx.x - before + grid) % grid;
+      before = (before + items) % grid;
+      for (int it = first; it < items; it += grid) {
+        const bool is_v = it & 1;
+        const int g = (it >> 1) % n_kv_heads, i = (it >> 1) / n_kv_heads;
+        const int logical = i < n_kept ? i : lo_page + i - n_kept;
+        const int page = logical < table_width ? block_table[(size_t)s_slot[s] * table_width + logical] : -1;
+        if (page < 0 || page >= n_pages) {
+          if (status && threadIdx.x == 0) atomicOr(status, FG_STATUS_BAD_PAGE);
+          continue;
+        }
+        if (!waited) {
+          pdl_wait();
+          waited = true;
+        }
+        const size_t block = (size_t)page * n_kv_heads + g;
+        const float scale = __uint_as_float(ld_global_4((is_v ? v_scales : k_scales) + block));
+        expand_block<HD>((is_v ? v_pages : k_pages) + block * bytes, (is_v ? v_out : k_out) + block * bytes, scale, page_size,
+                         is_v, 0, last - logical * page_size + 1);
+      }
+    }
+  }
+  if (!waited) pdl_wait();
+}
+
+}  // namespace fg_kv8

@@ -10,6 +10,7 @@ here falls back to the CPU or to eager PyTorch.
 from __future__ import annotations
 
 import ctypes
+import dataclasses
 import os
 from ctypes import c_float, c_int, c_ulonglong, c_void_p
 from typing import Optional
@@ -93,6 +94,7 @@ _CORE_SIGNATURES = {
     "fg_sample_uniform": [c_ulonglong, _P, _P, _P, _I, _P],
     "fg_set_table_entries": [_P, _P, _P, _I, _P],
     "fg_make_kv_tensor_map": [_P, _P, _I, _I, _I, _I, _I, _I],
+    "fg_make_kv8_tensor_map": [_P, _P, _I, _I, _I, _I, _I, _I],
 }
 
 _ATTN_SIGNATURES = {
@@ -235,6 +237,15 @@ _RECUR_SIGNATURES = {
     "fg_rglru_scan": [_P, _I, _P, _L, _I, _P, _P, _P, _P, _P, _L, _P, _L, _I, _P, _L, _L, _P, _P, _P, _I, _I, _I, _I,
                       _P],
 }
+_KV8_SIGNATURES = {
+    "fg_kv8_write": [_P, _I, _P, _P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P,
+                     _P, _P, _P, _I, _F, _I, _P],
+    "fg_kv8_values": [_P, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _P, _P],
+    "fg_kv8_expand": [_P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P],
+    "fg_kv8_attention_decode": [_P, _I, _P, _I, _P, _P, _I, _P, _P, _P, _I, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _F, _F, _P,
+                                ctypes.c_longlong, _I, ctypes.c_longlong, _P, _P, _P, _P],
+}
+_kv8 = {}
 _delta = None
 _moe = None
 _recur = None
@@ -299,6 +310,38 @@ def attn(head_dim: int):
     return lib
 
 
+def kv8(head_dim: int):
+    """The library of the paged cache in 8 bits for this head size."""
+    lib = _kv8.get(head_dim)
+    if lib is None:
+        lib = build.kv8_library(head_dim)
+        _declare(lib, _KV8_SIGNATURES)
+        lib.fg_kv8_decode_scratch_floats.argtypes = [_I, ctypes.c_longlong]
+        lib.fg_kv8_decode_scratch_floats.restype = ctypes.c_longlong
+        _kv8[head_dim] = lib
+    return lib
+
+
+class _PromptsOnly:
+    """A step's context without its single tokens."""
+
+    def __init__(self, ctx) -> None:
+        self._ctx = ctx
+
+    def __getattr__(self, name):
+        return getattr(self._ctx, name)
+
+    def single_tokens(self):
+        return _NO_SINGLES
+
+
+class _NoSingles:
+    n = 0
+
+
+_NO_SINGLES = _NoSingles()
+
+
 def require_cuda(device) -> torch.device:
     device = torch.device(device)
     if device.type != "cuda":
@@ -361,6 +404,9 @@ class Ops:
         # captured graphs may hold their addresses
         self._split = {}
         self._split_retired = []
+        # (pages, kv heads, page, head size) of an 8-bit cache -> its pages in bfloat16 as prompt portions read
+        # them (keys, values, tensor maps); every layer and group of these sizes fills the same pool in turn
+        self._expanded = {}
         self._latent_maps = {}  # (address, shape, box) of a layer's latent pool -> its tensor map
         self.use_tcgen05 = not bool(os.environ.get("FG_NO_TCGEN05"))
         # library products accumulate and reduce in float32 (no bfloat16 split-K sums)
@@ -1389,7 +1435,13 @@ class Ops:
         ``sinks`` (float32 [heads] or ``None``): ``exp(sinks[h])`` joins the softmax's denominator of head
         ``h`` once; it has no key and no value and is not scaled.
 
-        ``chunk`` (excludes a window): a query sees only the keys of its own chunk of that many positions."""
+        ``chunk`` (excludes a window): a query sees only the keys of its own chunk of that many positions.
+
+        A ``memory`` with scales is a cache in 8 bits (bfloat16 only): single tokens in a kernel of their own, for prompt
+        portions the pages they read are expanded to bfloat16 (exactly) and the kernels above run on those."""
+        if memory.k_scales is not None:
+            return self._attention_kv8(q, out, memory, ctx, n_heads, n_kv_heads, head_dim, window, scale, out_freqs,
+                                       keep_first, softcap, sinks, chunk)
         lib = attn(head_dim)
         assert not (window and chunk)
         window = -int(chunk) if chunk else int(window or 0)  # (see first_visible in common.cuh)
@@ -1492,6 +1544,152 @@ class Ops:
                     _ptr(q), q.stride(0), _ptr(out), out.stride(0), *common, *head, turn, float(softcap or 0.0),
                     _ptr(sinks), _ptr(self.status), _stream()))
             Ops.launches += 1  # the combine kernel
+        return fused
+
+    # -- the cache in 8 bits -------------------------------------------------------------------------
+    @staticmethod
+    def kv8_supported(head_dim: int, page_size: int) -> Optional[str]:
+        """``None``, or why a cache of these sizes cannot be held in 8 bits."""
+        if head_dim not in build.KV8_HEAD_DIMS:
+            return f"head size {head_dim} is not one of {build.KV8_HEAD_DIMS}"
+        if not 16 <= page_size <= 256 or page_size & (page_size - 1):
+            return f"pages of {page_size} tokens are not a power of two from 16 to 256"
+        return None
+
+    def _check_kv8(self, memory, n_kv_heads: int, head_dim: int) -> None:
+        why = self.kv8_supported(head_dim, memory.page_size)
+        if why is not None:
+            raise ValueError(f"a cache in 8 bits: {why}")
+        if self.act_dtype != torch.bfloat16:
+            raise ValueError("a cache in 8 bits serves bfloat16 models")
+        n_pages, page = memory.k_pages.shape[0], memory.page_size
+        for t, shape in ((memory.k_pages, (n_pages, n_kv_heads, page, head_dim)),
+                         (memory.v_pages, (n_pages, n_kv_heads, page // 4, head_dim, 4))):
+            if t.dtype != torch.float8_e4m3fn or tuple(t.shape) != shape or not t.is_contiguous():
+                raise ValueError(f"pages of a cache in 8 bits are contiguous e4m3 codes {shape}, got {t.dtype} {tuple(t.shape)}")
+        for t in (memory.k_scales, memory.v_scales):
+            if t.dtype != torch.float32 or tuple(t.shape) != (n_pages, n_kv_heads) or not t.is_contiguous():
+                raise ValueError(f"scales of a cache in 8 bits are contiguous float32 {(n_pages, n_kv_heads)}, "
+                                 f"got {t.dtype} {tuple(t.shape)}")
+
+    def make_kv8_tensor_maps(self, k_pool, v_pool):
+        """Tensor maps of the pools of a cache in 8 bits: codes ``[layers, pages, kv heads, page, head size]`` of keys and
+        ``[layers, pages, kv heads, page / 4, head size, 4]`` of values."""
+        n_layers, n_pages, n_kv_heads, page, head_dim = k_pool.shape
+        why = self.kv8_supported(head_dim, page)
+        if why is not None:
+            raise ValueError(f"a cache in 8 bits: {why}")
+        assert v_pool.shape == (n_layers, n_pages, n_kv_heads, page // 4, head_dim, 4)
+        maps = []
+        for pool in (k_pool, v_pool):
+            assert pool.dtype == torch.float8_e4m3fn and pool.is_contiguous()
+            tm = TensorMap()
+            _check(self.lib, self.lib.fg_make_kv8_tensor_map(
+                tm.ptr, _ptr(pool), n_layers, n_pages, n_kv_heads, page, head_dim, min(page, DECODE_SPLIT)))
+            Ops.launches -= 1  # not a kernel
+            maps.append(tm)
+        return tuple(maps)
+
+    def rope_kv8_write(self, q, k, v, pos, req, freqs, memory, n_heads: int, n_kv_heads: int, head_dim: int,
+                       v_freqs=None, qk_norm=None, magnitude: float = 1.0, rot_pairs: int = 0) -> torch.Tensor:
+        """:meth:`rope_kv_write` for a cache in 8 bits: returns the rotated queries [T, heads * head size] and writes
+        rotated keys and values to their pages as e4m3 codes with one power of two a (page, head), the smallest ``2^e``
+        (``e >= -100``) at which every magnitude is at most ``448 * 2^e``.  Tokens that begin a page choose it; tokens
+        behind cached ones never lower it, and where they raise it the cached codes are rounded again.  A sequence's
+        tokens are neighbours in the step and in ascending order.  Entries that are not finite are stored as NaN.
+        Queries, keys and values are bfloat16; the rotated numbers are rounded once, to their codes."""
+        self._check_kv8(memory, n_kv_heads, head_dim)
+        t = q.shape[0]
+        for x, heads in ((q, n_heads), (k, n_kv_heads), (v, n_kv_heads)):
+            if x.dtype != torch.bfloat16 or x.stride(1) != 1 or tuple(x.shape) != (t, heads * head_dim):
+                raise ValueError(f"rope_kv8_write takes bfloat16 rows of {heads} heads of {head_dim}, got {x.dtype} {tuple(x.shape)}")
+        if n_heads % n_kv_heads:
+            raise ValueError(f"{n_heads} heads over {n_kv_heads} key/value heads")
+        assert pos.dtype == torch.int32 and req.dtype == torch.int32 and pos.numel() == req.numel() == t
+        table = memory.block_table
+        assert table.dtype == torch.int32 and table.is_contiguous()
+        for f in (freqs, v_freqs):
+            assert f is None or (f.dtype == torch.float32 and f.numel() == head_dim // 2 and f.is_contiguous())
+        rstd, qn_w, kn_w = qk_norm if qk_norm is not None else (None, None, None)
+        rstd_heads = 0
+        if rstd is not None:
+            assert rstd.dtype == torch.float32 and rstd.is_contiguous() and rstd.shape[0] == t
+            rstd_heads = 0 if rstd.shape[1] == 2 else rstd.shape[1]
+            assert rstd_heads in (0, n_heads + n_kv_heads)
+            assert qn_w is None or (qn_w.dtype == torch.float32 and qn_w.numel() == n_heads * head_dim and qn_w.is_contiguous())
+            assert kn_w is None or (kn_w.dtype == torch.float32 and kn_w.numel() == n_kv_heads * head_dim and kn_w.is_contiguous())
+        out = torch.empty((t, n_heads * head_dim), dtype=torch.bfloat16, device=q.device)
+        lib = kv8(head_dim)
+        _check(lib, lib.fg_kv8_write(
+            _ptr(q), q.stride(0), _ptr(out), _ptr(k), k.stride(0), _ptr(v), v.stride(0), _ptr(pos), _ptr(req), _ptr(freqs),
+            _ptr(v_freqs), _ptr(memory.k_pages), _ptr(memory.v_pages), _ptr(memory.k_scales), _ptr(memory.v_scales),
+            _ptr(table), table.shape[1], memory.page_size, memory.k_pages.shape[0], t, n_heads, n_kv_heads, head_dim,
+            _ptr(self.status), _ptr(rstd), _ptr(qn_w), _ptr(kn_w), rstd_heads, float(magnitude), int(rot_pairs), _stream()))
+        return out
+
+    def kv8_values(self, memory, pages):
+        """What the pages ``pages`` (int32, on the device) of a cache in 8 bits stand for: keys and values in bfloat16
+        ``[n, kv heads, page, head size]``, every slot of the pages, also those that hold no token."""
+        n_pages, n_kv_heads, page, head_dim = memory.k_pages.shape
+        self._check_kv8(memory, n_kv_heads, head_dim)
+        assert pages.dtype == torch.int32 and pages.is_contiguous()
+        k = torch.empty((pages.numel(), n_kv_heads, page, head_dim), dtype=torch.bfloat16, device=pages.device)
+        v = torch.empty_like(k)
+        lib = kv8(head_dim)
+        _check(lib, lib.fg_kv8_values(
+            _ptr(memory.k_pages), _ptr(memory.v_pages), _ptr(memory.k_scales), _ptr(memory.v_scales), _ptr(pages), pages.numel(),
+            _ptr(k), _ptr(v), page, n_pages, n_kv_heads, head_dim, _ptr(self.status), _stream()))
+        return k, v
+
+    def kv8_expanded(self, memory):
+        """The pool that prompt portions over a cache of this shape read: keys and values in bfloat16 and their tensor
+        maps.  Made at the first call (not inside a graph capture) and kept."""
+        key = tuple(memory.k_pages.shape)
+        got = self._expanded.get(key)
+        if got is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the first prompt portion over a cache in 8 bits cannot be inside a graph capture")
+            k = torch.zeros(key, dtype=torch.bfloat16, device=memory.k_pages.device)
+            v = torch.zeros_like(k)
+            got = self._expanded[key] = (k, v, self.make_kv_tensor_maps(k[None], v[None], key[2]))
+        return got
+
+    def _attention_kv8(self, q, out, memory, ctx, n_heads, n_kv_heads, head_dim, window, scale, out_freqs, keep_first,
+                       softcap, sinks, chunk) -> bool:
+        self._check_kv8(memory, n_kv_heads, head_dim)
+        assert q.dtype == torch.bfloat16 and out.dtype == torch.bfloat16 and q.stride(1) == 1 and out.stride(1) == 1
+        assert not (window and chunk)
+        assert sinks is None or (sinks.dtype == torch.float32 and sinks.numel() == n_heads and sinks.is_contiguous())
+        if window and keep_first:
+            raise ValueError("a cache in 8 bits knows no window that keeps first positions")
+        table = memory.block_table
+        lib = kv8(head_dim)
+        signed_window = -int(chunk) if chunk else int(window or 0)
+        n_pages, page = memory.k_pages.shape[0], memory.page_size
+        singles = ctx.single_tokens()
+        prompts = ctx.attention_tiles(attention_tiling(n_heads, n_kv_heads, PREFILL_TMA_ROWS), 2).n > 0
+        if prompts:
+            k, v, maps = self.kv8_expanded(memory)
+            _check(lib, lib.fg_kv8_expand(
+                _ptr(memory.k_pages), _ptr(memory.v_pages), _ptr(memory.k_scales), _ptr(memory.v_scales), _ptr(table),
+                table.shape[1], _ptr(ctx.seq_slot), _ptr(ctx.seq_start), _ptr(ctx.seq_cached), ctx.n_seqs, _ptr(k), _ptr(v), page,
+                n_pages, n_kv_heads, head_dim, signed_window, 0, _ptr(self.status), _stream()))
+            expanded = dataclasses.replace(memory, k_pages=k, v_pages=v, k_scales=None, v_scales=None, tensor_maps=maps,
+                                           layer_index=0)
+            self.attention(q, out, expanded, _PromptsOnly(ctx), n_heads, n_kv_heads, head_dim, window, scale,
+                           softcap=softcap, sinks=sinks, chunk=chunk)
+        fused = out_freqs is not None and not prompts and singles.n > 0
+        if singles.n:
+            max_splits = max(1, -(-singles.max_len // DECODE_SPLIT))
+            pairs = min(singles.n * max_splits, singles.stretches(DECODE_SPLIT))
+            scratch = self._decode_scratch(lib.fg_kv8_decode_scratch_floats(n_heads, pairs))
+            _check(lib, lib.fg_kv8_attention_decode(
+                _ptr(q), q.stride(0), _ptr(out), out.stride(0), memory.tensor_maps[0].ptr, memory.tensor_maps[1].ptr,
+                memory.layer_index, _ptr(memory.k_scales), _ptr(memory.v_scales), _ptr(table), table.shape[1], page, n_pages,
+                _ptr(ctx.pos), _ptr(singles.req), _ptr(singles.tok), singles.n, n_heads, n_kv_heads, head_dim, signed_window,
+                float(scale), float(softcap or 0.0), _ptr(scratch), scratch.numel(), max_splits, pairs,
+                _ptr(out_freqs) if fused else None, _ptr(sinks), _ptr(self.status), _stream()))
+            Ops.launches += 1  # the merge
         return fused
 
     def rotate_heads(self, x, pos, req, freqs, n_heads: int, head_dim: int) -> torch.Tensor:

@@ -56,3 +56,22 @@ extern "C" int fg_make_kv_tensor_map(void* out_map, const void* base, int n_laye
   return fg_encode_tensor_map(reinterpret_cast<CUtensorMap*>(out_map), CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, base, dims,
                               strides, box);
 }
+
+// A pool of the cache in 8 bits (keys or values): its (layer, page, head) blocks as lines of 128 bytes, a box of box_rows
+// slots of one block.
+extern "C" int fg_make_kv8_tensor_map(void* out_map, const void* base, int n_layers, int n_pages, int n_kv_heads,
+                                      int page_size, int head_dim, int box_rows) {
+  FG_CHECK_ARG(((uintptr_t)out_map & 63) == 0, "fg_make_kv8_tensor_map: the map must be 64-byte aligned");
+  FG_CHECK_ARG(((uintptr_t)base & 15) == 0, "fg_make_kv8_tensor_map: the pool must be 16-byte aligned");
+  FG_CHECK_ARG(head_dim == 64 || head_dim == 128 || head_dim == 256, "fg_make_kv8_tensor_map: head size %d is not 64, 128 or 256",
+               head_dim);
+  FG_CHECK_ARG(box_rows > 0 && box_rows <= page_size && box_rows * head_dim % 128 == 0 && box_rows * head_dim / 128 <= 256,
+               "fg_make_kv8_tensor_map: bad box of %d rows for pages of %d", box_rows, page_size);
+  const cuuint64_t blocks = (cuuint64_t)n_layers * n_pages * n_kv_heads;
+  FG_CHECK_ARG(blocks > 0 && blocks <= 0x7fffffffull, "fg_make_kv8_tensor_map: %llu blocks", (unsigned long long)blocks);
+  const cuuint64_t bytes = (cuuint64_t)page_size * head_dim;
+  const cuuint64_t dims[3] = {128, bytes / 128, blocks};
+  const cuuint64_t strides[2] = {128, bytes};
+  const cuuint32_t box[3] = {128, (cuuint32_t)(box_rows * head_dim / 128), 1};
+  return fg_encode_tensor_map(reinterpret_cast<CUtensorMap*>(out_map), CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, base, dims, strides, box);
+}
