@@ -53,6 +53,7 @@ CORE_SOURCES = [
     "gemm_f32.cu",
     "gemm_f32_split.cu",
     "gemm_skinny.cu",
+    "gemm_w4.cu",
     "sampling.cu",
     "tensor_map.cu",
     "table_entries.cu",

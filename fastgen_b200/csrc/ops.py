@@ -18,6 +18,7 @@ from typing import Optional
 import numpy as np
 import torch
 
+from ..weights.four_bit import Weight4
 from . import build
 
 FG_F32, FG_BF16 = 0, 1
@@ -89,6 +90,7 @@ _CORE_SIGNATURES = {
     "fg_gemm_skinny_swiglu_bf16": [_P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _P],
     "fg_gemm_skinny_qkv_bf16": [_P, _I, _P, _I, _P, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I,
                                 _I, _I, _P, _P],
+    "fg_gemm_w4": [_P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _P, _I, _I, _P],
     "fg_sample": [_P, _I, _I, _I, _P, _F, c_ulonglong, _P, _P, _P, _P, _P, _P, _P],
     "fg_selftest_wait_timeout": [_I, _P, _P, _P],
     "fg_sample_uniform": [c_ulonglong, _P, _P, _P, _I, _P],
@@ -128,6 +130,7 @@ _ATTN_SIGNATURES = {
 }
 
 SKINNY_MAX_M = int(os.environ.get("FG_SKINNY_MAX_M", "8"))      # most tokens the weight-streaming product is used for (it takes up to 32)
+W4_MAX_M = 16        # tokens a launch of the product that streams 4-bit weights takes
 SIMT_ROWS = 16       # query rows per block of the float32 attention kernel
 F32_PROMPT_ROWS = 64  # ... of the float32 kernel of larger prompts
 PREFILL_ROWS = 64    # ... of the bfloat16 prompt kernel
@@ -1073,7 +1076,11 @@ class Ops:
                act: Optional[str] = None) -> torch.Tensor:
         """``act(x @ w.T + bias)`` for ``x`` [M, K] and ``w`` [N, K] (fastgen/forward.py:438-440);
         ``bias`` [N] of the compute dtype and ``act`` (a key of ``ACTIVATIONS``) are optional.  The
-        bias is added to the float32 sums; the activation sees the rounded result."""
+        bias is added to the float32 sums; the activation sees the rounded result.  ``w`` may be a
+        :class:`~fastgen_b200.weights.Weight4` (bfloat16 only): its whole numbers enter the product as they are and a
+        group's float32 sums are multiplied by its scale."""
+        if isinstance(w, Weight4):
+            return self._linear4(x, w, out, out_dtype, bias, act)
         m, k = x.shape
         n = w.shape[0]
         assert w.shape[1] == k and x.stride(1) == 1 and w.stride(1) == 1
@@ -1128,6 +1135,28 @@ class Ops:
             out.copy_(res)
             return out
         return res
+
+    def _linear4(self, x, w: Weight4, out=None, out_dtype=None, bias=None, act=None, gated: bool = False) -> torch.Tensor:
+        """The product with 4-bit weights.  ``gated``: the rows of ``w`` are gate and up in blocks of 8 in turn, ``act`` a key of
+        ``GATES``, and the result is the gated half."""
+        (m, k), (n, wk) = x.shape, w.shape
+        if self.act_dtype != torch.bfloat16 or x.dtype != torch.bfloat16:
+            raise ValueError(f"4-bit weights take bfloat16 activations, got {x.dtype}")
+        if wk != k or x.stride(1) != 1:
+            raise ValueError(f"a product of {tuple(x.shape)} with 4-bit weights {w.shape}")
+        if bias is not None and (bias.shape != (n,) or bias.dtype != torch.bfloat16 or not bias.is_contiguous()):
+            raise ValueError(f"the bias of {n} rows is contiguous bfloat16, got {bias.dtype} {tuple(bias.shape)}")
+        if x.stride(0) % 8 or x.data_ptr() % 16:
+            x = x.contiguous() if not x.is_contiguous() else x.clone()  # rows off 16 bytes (k is a multiple of 32)
+        if out is None:
+            out = torch.empty((m, n // 2 if gated else n), dtype=out_dtype or torch.bfloat16, device=x.device)
+        assert out.stride(1) == 1 and tuple(out.shape) == (m, n // 2 if gated else n)
+        code = GATES[act or "silu"] if gated else ACTIVATIONS[act]
+        for i in range(0, m, W4_MAX_M):
+            _check(self.lib, self.lib.fg_gemm_w4(
+                _ptr(x[i:]), x.stride(0), _ptr(w.packed), _ptr(w.scales), w.group, _ptr(out[i:]), out.stride(0), _code(out.dtype),
+                min(W4_MAX_M, m - i), n, k, _ptr(bias), code, int(gated), _stream()))
+        return out
 
     def _skinny_ok(self, x: torch.Tensor, w: torch.Tensor, k: int) -> bool:
         return (x.dtype == torch.bfloat16 and x.shape[0] <= SKINNY_MAX_M and k % 8 == 0
