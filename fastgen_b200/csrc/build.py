@@ -54,6 +54,7 @@ CORE_SOURCES = [
     "gemm_f32_split.cu",
     "gemm_skinny.cu",
     "gemm_w4.cu",
+    "gemm_w4_tc5.cu",
     "sampling.cu",
     "tensor_map.cu",
     "table_entries.cu",

@@ -91,6 +91,7 @@ _CORE_SIGNATURES = {
     "fg_gemm_skinny_qkv_bf16": [_P, _I, _P, _I, _P, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I,
                                 _I, _I, _P, _P],
     "fg_gemm_w4": [_P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _P, _I, _I, _P],
+    "fg_gemm_w4_tc5": [_P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _P, _I, _I, _I, _P, _P],
     "fg_sample": [_P, _I, _I, _I, _P, _F, c_ulonglong, _P, _P, _P, _P, _P, _P, _P],
     "fg_selftest_wait_timeout": [_I, _P, _P, _P],
     "fg_sample_uniform": [c_ulonglong, _P, _P, _P, _I, _P],
@@ -1152,10 +1153,14 @@ class Ops:
             out = torch.empty((m, n // 2 if gated else n), dtype=out_dtype or torch.bfloat16, device=x.device)
         assert out.stride(1) == 1 and tuple(out.shape) == (m, n // 2 if gated else n)
         code = GATES[act or "silu"] if gated else ACTIVATIONS[act]
-        for i in range(0, m, W4_MAX_M):
+        if m <= W4_MAX_M:
             _check(self.lib, self.lib.fg_gemm_w4(
-                _ptr(x[i:]), x.stride(0), _ptr(w.packed), _ptr(w.scales), w.group, _ptr(out[i:]), out.stride(0), _code(out.dtype),
-                min(W4_MAX_M, m - i), n, k, _ptr(bias), code, int(gated), _stream()))
+                _ptr(x), x.stride(0), _ptr(w.packed), _ptr(w.scales), w.group, _ptr(out), out.stride(0), _code(out.dtype),
+                m, n, k, _ptr(bias), code, int(gated), _stream()))
+        else:
+            _check(self.lib, self.lib.fg_gemm_w4_tc5(
+                _ptr(x), x.stride(0), _ptr(w.packed), _ptr(w.scales), w.group, _ptr(out), out.stride(0), _code(out.dtype),
+                m, n, k, _ptr(bias), code, int(gated), 0, _ptr(self.status), _stream()))
         return out
 
     def _skinny_ok(self, x: torch.Tensor, w: torch.Tensor, k: int) -> bool:
