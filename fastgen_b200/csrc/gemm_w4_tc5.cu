@@ -15,6 +15,8 @@
 //
 // What bounds it: few tokens: reading the codes; the workers' instructions (11 for eight weights) come to about two thirds of
 // what the SM issues meanwhile.
+#include <type_traits>
+
 #include "skinny_product.cuh"
 #include "tc5_primitives.cuh"
 #include "tensor_map.cuh"
@@ -40,7 +42,7 @@ struct Shape4 {
   static constexpr int TMEM = COL_D + D_BUFS * D_COLS <= 256 ? 256 : 512;
   static constexpr int BLOCKS = TMEM == 256 && T <= 64 ? 2 : 1;  // an SM
   static constexpr int W_STAGES = T <= 32 ? 4 : BLOCKS == 2 ? 3 : 4;
-  static constexpr int X_UNITS = 4;
+  static constexpr int X_UNITS = T == 64 ? 3 : 4;
   static constexpr int RINGS = W_STAGES * W_STAGE + X_UNITS * X_UNIT;
   // The blocks of a cluster wait for one another, so none of them may wait for tensor memory that a block of another
   // cluster keeps meanwhile: shared memory is asked for such that an SM holds no more blocks, of any of these
@@ -253,53 +255,54 @@ gemm_w4_tc5_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
     float acc[TC];
 #pragma unroll
     for (int i = 0; i < TC; ++i) acc[i] = 0.f;
-    int slot = 0, use = 0;
-    __nv_bfloat16 sc_next[PARTS];
-    float sc[PARTS];
     share_tmem();
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
-    for (int j = 0; j <= total; ++j) {
+    const __nv_bfloat16* next_scale = my_scales + k_begin / S::G;
+    __nv_bfloat16 sc_next[PARTS];
+    float sc[PARTS];
+    // pieces of 16 bytes (32 codes) of this thread's row in a stage, swizzled: chunk c's two for this half of the columns
+    const unsigned char* my_row = ws + row * 128;
+    int piece_at[2][2];
 #pragma unroll
-      for (int p = 0; p < PARTS; ++p) sc[p] = j > 0 ? __bfloat162float(sc_next[p]) : 0.f;
-      if (j < total) {
-        const int buf = j & 1, k0 = k_begin + j * KC;
+    for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p)
-          sc_next[p] = k0 + p * S::G < K ? my_scales[k0 / S::G + p] : __float2bfloat16_rn(0.f);
-        if ((j & 1) == 0) mbar_wait(&w_full[slot], use & 1, status, &gave_up);
-        const unsigned char* src = ws + slot * W_STAGE + row * 128;
-        uint4 codes[2];
+      for (int i = 0; i < 2; ++i) piece_at[c][i] = ((c * 4 + half * 2 + i) ^ (row & 7)) << 4;
+    const uint32_t op0 = tmem + my_lane + S::COL_A + half * 32, d0 = tmem + my_lane + S::COL_D + half * TC;
+
+    // a chunk's codes (the stage's chunk PARITY) -> tensor memory; the sums of the chunk before it -> acc
+    auto expand = [&](auto parity_tag, int j, int slot) {
+      constexpr int PARITY = decltype(parity_tag)::value;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          codes[i] = *reinterpret_cast<const uint4*>(src + ((((j & 1) * 4 + half * 2 + i) ^ (row & 7)) << 4));
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
-          uint32_t v[16];
-#pragma unroll
-          for (int c = 0; c < 16; ++c) v[c] = weights_of(w[c >> 2], c & 3);
-          tmem_st16(tmem + my_lane + S::COL_A + buf * A_COLS + half * 32 + i * 16, v);
-        }
-        if ((j & 1) == 1 || j + 1 == total) {
-          warp_arrive(&w_empty[slot]);
-          if (++slot == S::W_STAGES) {
-            slot = 0;
-            ++use;
-          }
-        }
-        tmem_st_wait();
-        tc_fence_before();
-        warp_arrive(&op_full[buf]);
+      for (int p = 0; p < PARTS; ++p) {
+        sc[p] = __bfloat162float(sc_next[p]);
+        // (groups of 128: every chunk is whole)
+        sc_next[p] = S::G == KC || k_begin + j * KC + p * S::G < K ? next_scale[p] : __float2bfloat16_rn(0.f);
       }
-      if (j == 0) continue;
-      // the sums of the chunk before
-      const int db = S::D_BUFS == 2 ? (j - 1) & 1 : 0, d_use = S::D_BUFS == 2 ? (j - 1) >> 1 : j - 1;
+      next_scale += PARTS;
+      uint4 codes[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) codes[i] = *reinterpret_cast<const uint4*>(my_row + slot * W_STAGE + piece_at[PARITY][i]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
+        uint32_t v[16];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) v[c] = weights_of(w[c >> 2], c & 3);
+        tmem_st16(op0 + PARITY * A_COLS + i * 16, v);
+      }
+      if (PARITY == 1) warp_arrive(&w_empty[slot]);
+      tmem_st_wait();
+      tc_fence_before();
+      warp_arrive(&op_full[PARITY]);
+    };
+    auto add_sums = [&](int j) {  // of chunk j
+      const int db = S::D_BUFS == 2 ? j & 1 : 0, d_use = S::D_BUFS == 2 ? j >> 1 : j;
       mbar_wait(&d_full[db], d_use & 1, status, &gave_up);
       tc_fence_after();
 #pragma unroll
       for (int p = 0; p < PARTS; ++p) {
-        const uint32_t d = tmem + my_lane + S::COL_D + db * S::D_COLS + p * T + half * TC;
+        const uint32_t d = d0 + db * S::D_COLS + p * T;
         constexpr int FLIGHT = TC < 32 ? TC : 32;  // columns in flight
 #pragma unroll
         for (int c = 0; c < TC; c += FLIGHT) {
@@ -315,40 +318,58 @@ gemm_w4_tc5_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
           for (int i = 0; i < FLIGHT; ++i) acc[c + i] = fmaf(__uint_as_float(v[i]), sc[p], acc[c + i]);
         }
       }
-    }
-    pdl_wait();  // y may still be read by the kernels before (over by now: its tensor memory was waited for)
-    if (share == 1) {
-      const float bias = epi.bias != nullptr && n < N ? __bfloat162float(epi.bias[n]) : 0.f;
+    };
+    int slot = 0, use = 0;
 #pragma unroll
-      for (int i = 0; i < TC; ++i) {
-        const int m = m0 + half * TC + i;
-        store_sum<TO>(acc[i], m, n, m < M, N, y, ldy, epi, bias);
+    for (int p = 0; p < PARTS; ++p) sc_next[p] = __float2bfloat16_rn(0.f);
+    for (int j = 0; j < total; j += 2) {
+      mbar_wait(&w_full[slot], use & 1, status, &gave_up);
+      expand(std::integral_constant<int, 0>(), j, slot);
+      if (j > 0) add_sums(j - 1);
+      if (j + 1 < total) {
+        expand(std::integral_constant<int, 1>(), j + 1, slot);
+        add_sums(j);
       }
-    } else {
-      // (every chunk of this block has been read out of the rings by now)
-      float* part = reinterpret_cast<float*>(ws);
-#pragma unroll
-      for (int i = 0; i < TC; ++i) part[(half * TC + i) * ROWS4 + row] = acc[i];
+      if (++slot == S::W_STAGES) {
+        slot = 0;
+        ++use;
+      }
     }
+    if (total > 0) {
+#pragma unroll
+      for (int p = 0; p < PARTS; ++p) sc[p] = __bfloat162float(sc_next[p]);
+      add_sums(total - 1);
+    }
+    // the sums to shared memory: every chunk of this block has been read out of the rings by now
+    float* part = reinterpret_cast<float*>(ws);
+#pragma unroll
+    for (int i = 0; i < TC; ++i) part[(half * TC + i) * ROWS4 + row] = acc[i];
+    if (share == 1) asm volatile("bar.sync 2, %0;\n" ::"n"(WORKERS) : "memory");
   }
-  if (share > 1) {
-    cluster_sync();
-    if (tid < WORKERS) {
-      // a warp 32 rows of W of one token, the cluster's warps in turn
-      const int tokens = min(T, M - m0);
-      for (int u = warp * share + rank; u < tokens * 4; u += 8 * share) {
-        const int i = u >> 2, r = (u & 3) * 32 + lane, n = n0 + r;
+  if (share > 1) cluster_sync();
+  if (tid < WORKERS) {
+    // a warp 32 rows of W of one token, the cluster's warps in turn (one loop for all of them: the activations' code once)
+    const int tokens = min(T, M - m0);
+#pragma unroll 1
+    for (int u = warp * share + rank; u < tokens * 4; u += 8 * share) {
+      const int i = u >> 2, r = (u & 3) * 32 + lane, n = n0 + r;
+      float v;
+      if (share == 1) {
+        v = reinterpret_cast<const float*>(ws)[i * ROWS4 + r];
+      } else {
         const uint32_t at = smem_u32(ws) + (i * ROWS4 + r) * 4;
         float p[8];
 #pragma unroll
         for (int s = 0; s < 8; ++s) p[s] = s < share ? ld_cluster(at, s) : 0.f;
-        float v = p[0];
+        v = p[0];
 #pragma unroll
         for (int s = 1; s < 8; ++s) v += p[s];
-        const float bias = epi.bias != nullptr && n < N ? __bfloat162float(epi.bias[n]) : 0.f;
-        store_sum<TO>(v, m0 + i, n, true, N, y, ldy, epi, bias);
       }
+      const float bias = epi.bias != nullptr && n < N ? __bfloat162float(epi.bias[n]) : 0.f;
+      store_sum<TO>(v, m0 + i, n, true, N, y, ldy, epi, bias);
     }
+  }
+  if (share > 1) {
     __syncwarp();
     cluster_sync();  // nobody leaves while its sums are being read
   }

@@ -112,7 +112,7 @@ extern "C" int fg_kv8_attention_decode(const void* q, int q_stride, void* out, i
   CUtensorMap km, vm;
   memcpy(&km, k_map, sizeof(CUtensorMap));
   memcpy(&vm, v_map, sizeof(CUtensorMap));
-  const size_t smem = decode_smem_bytes<FG_HEAD_DIM>(group, n_seqs);
+  const size_t smem = decode_smem_bytes<FG_HEAD_DIM>(n_seqs);
   auto kern = window < 0 ? kv8_decode_kernel<FG_HEAD_DIM, true> : kv8_decode_kernel<FG_HEAD_DIM, false>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   FG_CHECK_ARG(e == cudaSuccess, "fg_kv8_attention_decode: shared memory: %s", cudaGetErrorString(e));

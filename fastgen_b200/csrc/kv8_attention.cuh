@@ -1,9 +1,10 @@
 // Attention of single tokens over the cache in 8 bits.
 //
-// The scheme of the 16-bit cache's persistent kernel: blocks stay on their SM and walk the (request, split of 128 keys,
-// key/value head) items that exist; a producer warp streams codes through a ring of shared-memory slots, four consumer
-// warps take 32 keys each, partials per split go to scratch and attention_combine_kernel merges them.  What differs is
-// what 8 bits ask for:
+// Blocks stay on their SM and walk the (request, key/value head, split of 128 keys) items that exist, each block a stretch of
+// neighbours, so that a request's queries are converted once for many splits.  A producer warp streams codes through a ring
+// of shared-memory slots ahead of four consumer warps; partials per split go to scratch and attention_combine_kernel merges
+// them.  In the first product a consumer warp has 32 keys; the weights go to shared memory, and in the second product it
+// has a quarter of the dimensions of all 128 keys, so that there are no sums of warps to merge.
 //
 //  * Codes become half precision on their way into a fragment, which is exact, by one conversion for two codes; bfloat16
 //    operands would need four instructions for two.  Queries are bfloat16, whose range half precision does not have: a
@@ -47,18 +48,14 @@ constexpr float WEIGHT_SHIFT = 15.f;
 constexpr int NO_PAGE = -1000;       // in an exponent's place
 
 template <int HD>
-__host__ __device__ constexpr int decode_slots() { return HD == 64 ? 6 : HD == 128 ? 4 : 2; }
+__host__ __device__ constexpr int decode_slots() { return HD == 64 ? 6 : HD == 128 ? 4 : 3; }
 template <int HD>
-__host__ __device__ constexpr int decode_blocks_per_sm() { return HD == 64 ? 3 : 2; }
-template <int HD>
-__host__ __device__ constexpr int merge_ld() { return HD + 4; }
+__host__ __device__ constexpr int decode_blocks_per_sm() { return HD <= 128 ? 3 : 2; }
 
 template <int HD>
-inline size_t decode_smem_bytes(int group, int n_seqs) {
-  const int columns = group < MAX_COLUMNS ? group : MAX_COLUMNS;
-  // the ring, the merge buffer of the four warps (values, maxima, sums), positions and pair counts, alignment slack
-  return (size_t)decode_slots<HD>() * SPLIT * HD + (size_t)4 * columns * merge_ld<HD>() * 4 + 2 * 4 * MAX_COLUMNS * 4 +
-         (size_t)(2 * n_seqs + 1) * 4 + 1024;
+inline size_t decode_smem_bytes(int n_seqs) {
+  // the ring, positions and pair counts, alignment slack
+  return (size_t)decode_slots<HD>() * SPLIT * HD + (size_t)(2 * n_seqs + 1) * 4 + 1024;
 }
 
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
@@ -122,19 +119,20 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
                   float* __restrict__ scratch, long long max_pairs, int max_splits, int* status) {
   constexpr int SLOTS = decode_slots<HD>();
   constexpr int SLOT_BYTES = SPLIT * HD;
-  constexpr int MLD = merge_ld<HD>();
-  constexpr int KP = HD / 64, VP = HD / 32;  // 16-byte pieces a lane loads of a key's row and of a group of four values
+  constexpr int KP = HD / 64;               // 16-byte pieces a lane loads of a key's row
+  constexpr int VP = HD / 32;               // 16-byte pieces of a group of four values
+  constexpr int TILES = SPLIT / 16;         // tiles of 16 keys
+  constexpr int MINE = VP >= 4 ? VP / 4 : 1;  // pieces a warp has in the second product
+  constexpr int HALVES = VP >= 4 ? 2 : 1;     // products (of 16 dimensions) of a piece: a warp has both, or one at HD = 64
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* ring = reinterpret_cast<unsigned char*>(((uintptr_t)smem_unaligned + 1023) & ~(uintptr_t)1023);
-  const int columns = min(group, MAX_COLUMNS);
-  float* wo = reinterpret_cast<float*>(ring + SLOTS * SLOT_BYTES);  // [4 warps][columns][MLD]
-  float* wm = wo + 4 * columns * MLD;                               // [4][8] maxima
-  float* wl = wm + 4 * MAX_COLUMNS;                                 // [4][8] sums
-  int* s_pos = reinterpret_cast<int*>(wl + 4 * MAX_COLUMNS);        // [n_seqs] the token's position, -1: a padding lane
-  int* s_cum = s_pos + n_seqs;                                      // [n_seqs + 1] (request, split) pairs before it
+  int* s_pos = reinterpret_cast<int*>(ring + SLOTS * SLOT_BYTES);  // [n_seqs] the token's position, -1: a padding lane
+  int* s_cum = s_pos + n_seqs;                                     // [n_seqs + 1] (request, split) pairs before it
   __shared__ __align__(8) uint64_t full[SLOTS], empty[SLOTS];
-  __shared__ int s_exp[SLOTS][SPLIT / 16];  // exponents of the slot's boxes
-  __shared__ int gave_up;                   // set by a wait that ran out (see mbar_wait)
+  __shared__ int s_exp[SLOTS][2][TILES];     // exponents of the keys' and the values' boxes, with the keys' slot
+  __shared__ __align__(8) uint2 s_weights[TILES][32];  // the second product's right operand
+  __shared__ float s_top[4][MAX_COLUMNS], s_sum[4][MAX_COLUMNS];
+  __shared__ int gave_up;                    // set by a wait that ran out (see mbar_wait)
 
   pdl_trigger();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -172,35 +170,51 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
   __syncthreads();
 
   const int box_rows = min(page_size, SPLIT);
-  const int n_boxes = SPLIT / box_rows;
+  const int n_boxes = SPLIT / box_rows, box_shift = 31 - __clz(box_rows), page_shift = 31 - __clz(page_size);
   int n_pairs = s_cum[n_seqs];
   if (n_pairs > max_pairs) {
     // the scratch was sized for fewer: report instead of writing past it
     if (tid == 0 && blockIdx.x == 0 && status) atomicOr(status, FG_STATUS_BAD_SPLITS);
-    n_pairs = (int)max_pairs;
+    n_pairs = 0;
   }
-  // items: (request, split) pair, key/value head, slice of up to eight heads of its group
-  const int n_sub = (group + MAX_COLUMNS - 1) / MAX_COLUMNS;
-  const long long total = (long long)n_pairs * n_kv_heads * n_sub;
-  struct Item {
-    int pair, seq, g, sub, p, k0, k_begin;
+  // items: request, then (key/value head, slice of up to eight heads of its group), then split
+  const int n_sub = (group + MAX_COLUMNS - 1) / MAX_COLUMNS, slices = n_kv_heads * n_sub;
+  const long long total = (long long)n_pairs * slices;
+  const long long begin = total * blockIdx.x / gridDim.x;
+  const int count = (int)(total * (blockIdx.x + 1) / gridDim.x - begin);
+  struct Walk {
+    int seq, slice, split, n, p, first, k_begin;  // split counts from `first`, the request's first one; n of them
   };
-  auto item_of = [&](long long item) {
-    Item it;
-    it.sub = (int)(item % n_sub);
-    const long long r = item / n_sub;
-    it.g = (int)(r % n_kv_heads);
-    it.pair = (int)(r / n_kv_heads);
-    int lo = 0, hi = n_seqs;  // the last request whose first pair is <= pair
+  auto enter = [&](Walk& w) {
+    w.p = s_pos[w.seq];
+    w.first = first_split(w.p);
+    w.n = n_splits(w.p);
+    w.k_begin = first_visible<CHUNKS>(w.p, window);
+  };
+  auto start = [&]() {
+    Walk w{};
+    if (count == 0) return w;
+    int lo = 0, hi = n_seqs;  // the last request whose first item is <= begin
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (s_cum[mid] <= it.pair) lo = mid; else hi = mid;
+      if ((long long)s_cum[mid] * slices <= begin) lo = mid; else hi = mid;
     }
-    it.seq = lo;
-    it.p = s_pos[lo];
-    it.k0 = (first_split(it.p) + (it.pair - s_cum[lo])) * SPLIT;
-    it.k_begin = first_visible<CHUNKS>(it.p, window);
-    return it;
+    w.seq = lo;
+    enter(w);
+    const int in = (int)(begin - (long long)s_cum[lo] * slices);
+    w.slice = in / w.n;
+    w.split = in - w.slice * w.n;
+    return w;
+  };
+  // the next item; there is one
+  auto advance = [&](Walk& w) {
+    if (++w.split < w.n) return;
+    w.split = 0;
+    if (++w.slice < slices) return;
+    w.slice = 0;
+    do ++w.seq;
+    while (s_cum[w.seq + 1] == s_cum[w.seq]);
+    enter(w);
   };
 
   if (warp == 4) {
@@ -208,12 +222,12 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     // The step's own kernels write the page that holds the token's position (its cached entries may be rounded again at a
     // larger scale): splits that end before that page are loaded without waiting for them.
     bool waited = false;
-    auto page_of = [&](const Item& it) {  // lane i: the page of box i of the item's split, or -1
+    auto page_of = [&](const Walk& w) {  // lane i: the page of box i of the item's split, or -1
       int page = -1;
-      const int j0 = it.k0 + lane * box_rows;
-      if (lane < n_boxes && j0 <= it.p && j0 + box_rows > it.k_begin) {
-        const int logical = j0 / page_size;
-        page = logical < table_width ? block_table[(size_t)seq_req[it.seq] * table_width + logical] : -1;
+      const int j0 = (w.first + w.split) * SPLIT + lane * box_rows;
+      if (lane < n_boxes && j0 <= w.p && j0 + box_rows > w.k_begin) {
+        const int logical = j0 >> page_shift;
+        page = logical < table_width ? block_table[(size_t)seq_req[w.seq] * table_width + logical] : -1;
         if (page < 0 || page >= n_pages) {
           page = -1;
           if (status) atomicOr(status, FG_STATUS_BAD_PAGE);
@@ -221,141 +235,145 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
       }
       return page;
     };
-    int n_fill = 0;  // an item's keys are fill 2i, its values fill 2i + 1
-    Item it{};
-    int page = -1;
-    if ((long long)blockIdx.x < total) {
-      it = item_of(blockIdx.x);
-      page = page_of(it);
-    }
-    for (long long item = blockIdx.x; item < total; item += gridDim.x) {
-      if (!waited && it.k0 + SPLIT > (it.p & ~(page_size - 1))) {
+    Walk w = start();
+    int page = count > 0 ? page_of(w) : -1;
+    int slot = 0, use = 0;
+    for (int i = 0; i < count; ++i) {
+      const int k0 = (w.first + w.split) * SPLIT, g = w.slice / n_sub;
+      if (!waited && k0 + SPLIT > (w.p >> page_shift << page_shift)) {
         pdl_wait();
         waited = true;
       }
-      const size_t block = ((size_t)max(page, 0)) * n_kv_heads + it.g;
+      const size_t block = (size_t)max(page, 0) * n_kv_heads + g;
       const uint32_t ks = page >= 0 ? ld_global_4(k_scales + block) : 0u, vs = page >= 0 ? ld_global_4(v_scales + block) : 0u;
       // the next item's pages are on their way meanwhile
-      Item next{};
       int next_page = -1;
-      if (item + gridDim.x < total) {
-        next = item_of(item + gridDim.x);
-        next_page = page_of(next);
+      if (i + 1 < count) {
+        advance(w);
+        next_page = page_of(w);
       }
       const unsigned valid = __ballot_sync(0xffffffffu, page >= 0);
       const int bytes = __popc(valid) * box_rows * HD;
-      const int line0 = (it.k0 & (page_size - 1)) * HD / 128;  // 0 unless pages are longer than a split
+      const int line0 = (k0 & (page_size - 1)) * HD / 128;  // 0 unless pages are longer than a split
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
-        const int slot = n_fill % SLOTS;
-        if (n_fill >= SLOTS) mbar_wait(&empty[slot], (n_fill / SLOTS - 1) & 1, status, &gave_up);
-        if (lane < n_boxes) s_exp[slot][lane] = page >= 0 ? exponent_of_scale(__uint_as_float(kv ? vs : ks)) : NO_PAGE;
+        if (use > 0) mbar_wait(&empty[slot], (use - 1) & 1, status, &gave_up);
+        if (kv == 0 && lane < n_boxes) {
+          s_exp[slot][0][lane] = page >= 0 ? exponent_of_scale(__uint_as_float(ks)) : NO_PAGE;
+          s_exp[slot][1][lane] = page >= 0 ? exponent_of_scale(__uint_as_float(vs)) : 0;
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive_expect(&full[slot], bytes);
         __syncwarp();
         if (page >= 0)  // lane i issues box i's copy
           tma_load_3d(ring + slot * SLOT_BYTES + lane * box_rows * HD, kv ? &v_map : &k_map, 0, line0,
-                      (int)(((size_t)layer * n_pages + page) * n_kv_heads + it.g), &full[slot]);
-        ++n_fill;
+                      (int)(((size_t)layer * n_pages + page) * n_kv_heads + g), &full[slot]);
+        if (++slot == SLOTS) {
+          slot = 0;
+          ++use;
+        }
       }
-      it = next;
       page = next_page;
     }
     if (!waited) pdl_wait();
   } else {
     // ================================ consumers ================================
     pdl_wait();
-    int n_item = 0;
     const int g8 = lane >> 2, t4 = lane & 3;
-    for (long long item = blockIdx.x; item < total; item += gridDim.x) {
-      const Item it = item_of(item);
-      const int heads = min(MAX_COLUMNS, group - it.sub * MAX_COLUMNS);
-      const int head0 = it.g * group + it.sub * MAX_COLUMNS;
-      // the queries as the 8-column operand: column lane / 4 is a head, its elements in the order of the keys' pieces
-      uint32_t qb[KP][4][2];
-      float unscale;  // of head g8
-      {
-        const __nv_bfloat16* row = q + (size_t)seq_tok[it.seq] * q_stride + (head0 + min(g8, heads - 1)) * HD;
+    const int row_key = 4 * (g8 >> 1) + (g8 & 1);  // the key of row g8 of a tile; row g8 + 8 has that + 2
+    Walk w = start();
+    int slot = 0, use = 0;
+    bool fresh = true;
+    uint32_t qb[KP][4][2];
+    float un[2] = {1.f, 1.f};  // what undoes the queries' scaling, of the two heads whose scores this thread gets
+    int heads = 0, head0 = 0;
+    for (int i = 0; i < count; ++i) {
+      if (fresh) {
+        const int g = w.slice / n_sub, sub = w.slice - g * n_sub;
+        heads = min(MAX_COLUMNS, group - sub * MAX_COLUMNS);
+        head0 = g * group + sub * MAX_COLUMNS;
+        // the queries as the 8-column operand: column lane / 4 is a head, its elements in the order of the keys' pieces
+        const __nv_bfloat16* row = q + (size_t)seq_tok[w.seq] * q_stride + (head0 + min(g8, heads - 1)) * HD;
         uint4 raw[KP][2];
 #pragma unroll
-        for (int i = 0; i < KP; ++i) {
-          raw[i][0] = ld_global_16(row + 16 * key_piece<HD>(t4, i));
-          raw[i][1] = ld_global_16(row + 16 * key_piece<HD>(t4, i) + 8);
+        for (int c = 0; c < KP; ++c) {
+          raw[c][0] = ld_global_16(row + 16 * key_piece<HD>(t4, c));
+          raw[c][1] = ld_global_16(row + 16 * key_piece<HD>(t4, c) + 8);
         }
         uint32_t top = 0;  // the largest magnitude's bits: bfloat16 order is the order of its bits
 #pragma unroll
-        for (int i = 0; i < KP; ++i)
+        for (int c = 0; c < KP; ++c)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint32_t w[4] = {raw[i][h].x, raw[i][h].y, raw[i][h].z, raw[i][h].w};
+            const uint32_t x[4] = {raw[c][h].x, raw[c][h].y, raw[c][h].z, raw[c][h].w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) top = __vmaxu2(top, w[j] & 0x7fff7fffu);
+            for (int j = 0; j < 4; ++j) top = __vmaxu2(top, x[j] & 0x7fff7fffu);
           }
         int big = max(top & 0xffffu, top >> 16);
         big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
         big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
         const int up = min(14 - ((big >> 7) - 127), 126);  // power of two that the query is multiplied by
-        const float f = exp2_int(up);
-        unscale = exp2_int(-up);
+        const float f = exp2_int(up), unscale = exp2_int(-up);
 #pragma unroll
-        for (int i = 0; i < KP; ++i)
+        for (int c = 0; c < KP; ++c)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint32_t w[4] = {raw[i][h].x, raw[i][h].y, raw[i][h].z, raw[i][h].w};
+            const uint32_t x[4] = {raw[c][h].x, raw[c][h].y, raw[c][h].z, raw[c][h].w};
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              qb[i][2 * h + (j >> 1)][j & 1] =
-                  g8 < heads ? pack_f16(__uint_as_float(w[j] << 16) * f, __uint_as_float(w[j] & 0xffff0000u) * f) : 0u;
+              qb[c][2 * h + (j >> 1)][j & 1] =
+                  g8 < heads ? pack_f16(__uint_as_float(x[j] << 16) * f, __uint_as_float(x[j] & 0xffff0000u) * f) : 0u;
           }
+        un[0] = __shfl_sync(0xffffffffu, unscale, 8 * t4);
+        un[1] = __shfl_sync(0xffffffffu, unscale, 8 * t4 + 4);
       }
-      // of the two heads whose scores this thread gets
-      const float un[2] = {__shfl_sync(0xffffffffu, unscale, 8 * t4), __shfl_sync(0xffffffffu, unscale, 8 * t4 + 4)};
-      const int fk = 2 * n_item, fv = fk + 1;
-      const int slot_k = fk % SLOTS, slot_v = fv % SLOTS;
-      const unsigned char* Ks = ring + slot_k * SLOT_BYTES;
-      unsigned char* Vs = ring + slot_v * SLOT_BYTES;
+      const int k0 = (w.first + w.split) * SPLIT;
+      const bool edge = k0 < w.k_begin || k0 + SPLIT > w.p + 1;  // some keys of the split are not seen
+      const int last = w.p, k_begin = w.k_begin, pair = s_cum[w.seq] + w.split;
 
       // S^T[keys, heads] = K Q^T for this warp's 32 keys
-      mbar_wait(&full[slot_k], (fk / SLOTS) & 1, status, &gave_up);
+      const unsigned char* Ks = ring + slot * SLOT_BYTES;
+      mbar_wait(&full[slot], use & 1, status, &gave_up);
       float s[2][4];
-      int ek[2];
+      int ek[2], ev[2];
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
-        ek[mt] = s_exp[slot_k][(warp * 32 + mt * 16) / box_rows];
+        const int box = (warp * 32 + mt * 16) >> box_shift;
+        ek[mt] = s_exp[slot][0][box];
+        ev[mt] = s_exp[slot][1][box];
         s[mt][0] = s[mt][1] = s[mt][2] = s[mt][3] = 0.f;
-        const int key = warp * 32 + mt * 16 + 4 * (g8 >> 1) + (g8 & 1);
+        const int key = warp * 32 + mt * 16 + row_key;
 #pragma unroll
-        for (int i = 0; i < KP; ++i) {
-          const int piece = key_piece<HD>(t4, i);
+        for (int c = 0; c < KP; ++c) {
+          const int piece = key_piece<HD>(t4, c);
           const uint4 a = *reinterpret_cast<const uint4*>(Ks + key_offset<HD>(key, piece));
           const uint4 b = *reinterpret_cast<const uint4*>(Ks + key_offset<HD>(key + 2, piece));
           const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
           for (int m = 0; m < 4; ++m)
             mma_f16(s[mt], halves_of_low(aw[m]), halves_of_low(bw[m]), halves_of_high(aw[m]), halves_of_high(bw[m]),
-                    qb[i][m][0], qb[i][m][1]);
+                    qb[c][m][0], qb[c][m][1]);
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[slot_k]);  // this warp is done with the keys
+      if (lane == 0) mbar_arrive(&empty[slot]);  // this warp is done with the keys
+      if (++slot == SLOTS) {
+        slot = 0;
+        ++use;
+      }
 
       // this thread's scores: keys of row g8 and that + 2, heads 2 t4 and 2 t4 + 1
-      mbar_wait(&full[slot_v], (fv / SLOTS) & 1, status, &gave_up);
       float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
-      float fe[2];
-      const bool edge = it.k0 + warp * 32 < it.k_begin || it.k0 + warp * 32 + 31 > it.p || ek[0] == NO_PAGE || ek[1] == NO_PAGE;
+      const float fe[2] = {(float)ev[0], (float)ev[1]};
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
-        const int ev = s_exp[slot_v][(warp * 32 + mt * 16) / box_rows];
-        fe[mt] = (float)ev;
         const float ks = exp2_int(max(ek[mt], -126));
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float raw = s[mt][e] * un[e & 1] * ks;
-          float sc = capped_score(raw, scale_log2, cap_log2, scale_by_cap);
-          if (edge) {
-            const int j = it.k0 + warp * 32 + mt * 16 + 4 * (g8 >> 1) + (g8 & 1) + (e & 2);
-            if (j < it.k_begin || j > it.p || ek[mt] == NO_PAGE) sc = -INFINITY;
+          float sc = capped_score(s[mt][e] * un[e & 1] * ks, scale_log2, cap_log2, scale_by_cap);
+          if (edge || ek[mt] == NO_PAGE) {
+            const int j = k0 + warp * 32 + mt * 16 + row_key + (e & 2);
+            if (j < k_begin || j > last || ek[mt] == NO_PAGE) sc = -INFINITY;
           }
           s[mt][e] = sc;
           top[e & 1] = fmaxf(top[e & 1], sc + fe[mt]);
@@ -365,6 +383,14 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], o));
+      if (g8 == 0) *reinterpret_cast<float2*>(&s_top[warp][2 * t4]) = make_float2(top[0], top[1]);
+      asm volatile("bar.sync 1, %0;\n" ::"n"(CONSUMERS) : "memory");
+#pragma unroll
+      for (int o = 0; o < 4; ++o) {
+        const float2 other = *reinterpret_cast<const float2*>(&s_top[o][2 * t4]);
+        top[0] = fmaxf(top[0], other.x);
+        top[1] = fmaxf(top[1], other.y);
+      }
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
@@ -374,97 +400,89 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
           sum[e & 1] += ex2(x);
           s[mt][e] = ex2(x + fe[mt]);
         }
+      // the weights as the 8-column operand: an 8 x 8 transposition in registers for each half tile
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+        s_weights[warp * 2 + mt][lane] =
+            make_uint2(transposed_8x8(pack_f16(s[mt][0], s[mt][1])), transposed_8x8(pack_f16(s[mt][2], s[mt][3])));
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], o);
-      // the weights as the 8-column operand: an 8 x 8 transposition in registers for each half tile
-      uint32_t pb[2][2];
+      if (g8 == 0) *reinterpret_cast<float2*>(&s_sum[warp][2 * t4]) = make_float2(sum[0], sum[1]);
+      asm volatile("bar.sync 1, %0;\n" ::"n"(CONSUMERS) : "memory");
+
+      // O^T[dims, heads] = V^T P^T: this warp's pieces of all keys
+      const unsigned char* Vs = ring + slot * SLOT_BYTES;
+      mbar_wait(&full[slot], use & 1, status, &gave_up);
+      float o[MINE][HALVES][4];
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        pb[mt][0] = transposed_8x8(pack_f16(s[mt][0], s[mt][1]));
-        pb[mt][1] = transposed_8x8(pack_f16(s[mt][2], s[mt][3]));
-      }
-      if (edge) {
-        // codes of keys that are not seen: zero (a weight of zero times a NaN would be a NaN)
+      for (int c = 0; c < MINE; ++c)
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          const int grp = warp * 8 + mt * 4 + t4;
-          uint32_t mask = 0;
+        for (int h = 0; h < HALVES; ++h) o[c][h][0] = o[c][h][1] = o[c][h][2] = o[c][h][3] = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < TILES; ++mt) {
+        const uint2 pb = s_weights[mt][lane];
+        uint32_t mask = 0xffffffffu;
+        if (edge) {
+          // codes of keys that are not seen: zero (a weight of zero times a NaN of a page's former owner would be a NaN)
+          mask = 0;
 #pragma unroll
           for (int b = 0; b < 4; ++b) {
-            const int j = it.k0 + 4 * grp + b;
-            if (j >= it.k_begin && j <= it.p && ek[mt] != NO_PAGE) mask |= 0xffu << (8 * b);
-          }
-#pragma unroll
-          for (int i = 0; i < VP; ++i) {
-            uint4* at = reinterpret_cast<uint4*>(Vs + value_offset<HD>(grp, g8, i));
-            uint4 w = *at;
-            w.x &= mask, w.y &= mask, w.z &= mask, w.w &= mask;
-            *at = w;
+            const int j = k0 + mt * 16 + 4 * t4 + b;
+            if (j >= k_begin && j <= last) mask |= 0xffu << (8 * b);
           }
         }
-        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // the slot's next copy comes behind these stores
-      }
-
-      // O^T[dims, heads] = V^T P^T
-      float o[VP][2][4];
 #pragma unroll
-      for (int i = 0; i < VP; ++i) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) o[i][h][0] = o[i][h][1] = o[i][h][2] = o[i][h][3] = 0.f;
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          // dimensions 4 (g8 + 8 i) + 0..3 of the four keys of group t4 of the tile
-          const uint4 w = *reinterpret_cast<const uint4*>(Vs + value_offset<HD>(warp * 8 + mt * 4 + t4, g8, i));
-          mma_f16(o[i][0], halves_of_low(w.x), halves_of_low(w.y), halves_of_high(w.x), halves_of_high(w.y), pb[mt][0], pb[mt][1]);
-          mma_f16(o[i][1], halves_of_low(w.z), halves_of_low(w.w), halves_of_high(w.z), halves_of_high(w.w), pb[mt][0], pb[mt][1]);
+        for (int c = 0; c < MINE; ++c) {
+          // dimensions 4 (g8 + 8 i) + 0..3 of the four keys of group t4 of the tile; at HD = 64 a warp has two of the four
+          if constexpr (HALVES == 2) {
+            uint4 v = *reinterpret_cast<const uint4*>(Vs + value_offset<HD>(mt * 4 + t4, g8, warp + 4 * c));
+            if (edge) v.x &= mask, v.y &= mask, v.z &= mask, v.w &= mask;
+            mma_f16(o[c][0], halves_of_low(v.x), halves_of_low(v.y), halves_of_high(v.x), halves_of_high(v.y), pb.x, pb.y);
+            mma_f16(o[c][1], halves_of_low(v.z), halves_of_low(v.w), halves_of_high(v.z), halves_of_high(v.w), pb.x, pb.y);
+          } else {
+            uint2 v = *reinterpret_cast<const uint2*>(Vs + value_offset<HD>(mt * 4 + t4, g8, warp >> 1) + (warp & 1) * 8);
+            if (edge) v.x &= mask, v.y &= mask;
+            mma_f16(o[c][0], halves_of_low(v.x), halves_of_low(v.y), halves_of_high(v.x), halves_of_high(v.y), pb.x, pb.y);
+          }
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[slot_v]);  // ... and with the values
+      if (lane == 0) mbar_arrive(&empty[slot]);  // ... and with the values
+      if (++slot == SLOTS) {
+        slot = 0;
+        ++use;
+      }
 
-      // merge the four warps (heads of the item only)
-      if (g8 == 0) {
+      float* part = scratch + ((size_t)pair * n_heads + head0) * part_stride<HD>();
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          wm[warp * MAX_COLUMNS + 2 * t4 + h] = top[h];
-          wl[warp * MAX_COLUMNS + 2 * t4 + h] = sum[h];
-        }
+      for (int c = 0; c < MINE; ++c)
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            // rows g8 and g8 + 8 of the product are neighbouring dimensions
+            const int piece = HALVES == 2 ? warp + 4 * c : warp >> 1, which = HALVES == 2 ? h : warp & 1;
+            if (2 * t4 + e < heads)
+              *reinterpret_cast<float2*>(part + (2 * t4 + e) * part_stride<HD>() + 4 * (g8 + 8 * piece) + 2 * which) =
+                  make_float2(o[c][h][e], o[c][h][2 + e]);
+          }
+      if (warp == 0 && g8 == 0) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (2 * t4 + e < heads) {
+            float l = 0.f;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) l += s_sum[x][2 * t4 + e];
+            *reinterpret_cast<float2*>(part + (2 * t4 + e) * part_stride<HD>() + HD) = make_float2(top[e] - WEIGHT_SHIFT, l);
+          }
       }
-#pragma unroll
-      for (int i = 0; i < VP; ++i)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int head = 2 * t4 + c;
-          // rows g8 and g8 + 8 of the two products are neighbouring dimensions
-          if (head < heads)
-            *reinterpret_cast<float4*>(wo + (warp * columns + head) * MLD + 4 * (g8 + 8 * i)) =
-                make_float4(o[i][0][c], o[i][0][2 + c], o[i][1][c], o[i][1][2 + c]);
-        }
-      asm volatile("bar.sync 1, %0;\n" ::"n"(CONSUMERS) : "memory");
-      for (int i = tid; i < heads * HD; i += CONSUMERS) {
-        const int r = i / HD, d = i - r * HD;
-        float mm = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) mm = fmaxf(mm, wm[w * MAX_COLUMNS + r]);
-        float acc = 0.f, ll = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float mw = wm[w * MAX_COLUMNS + r];
-          const float f = (mw == -INFINITY) ? 0.f : ex2(mw - mm);
-          acc += f * wo[(w * columns + r) * MLD + d];
-          ll += f * wl[w * MAX_COLUMNS + r];
-        }
-        float* dst = scratch + ((size_t)it.pair * n_heads + head0 + r) * part_stride<HD>();
-        dst[d] = acc;
-        if (d == 0) {
-          dst[HD] = mm - WEIGHT_SHIFT;
-          dst[HD + 1] = ll;
-        }
+      if (i + 1 < count) {
+        const int seq = w.seq, slice = w.slice;
+        advance(w);
+        fresh = w.seq != seq || w.slice != slice;
       }
-      asm volatile("bar.sync 1, %0;\n" ::"n"(CONSUMERS) : "memory");  // the merge buffer is free again
-      ++n_item;
     }
   }
 }
