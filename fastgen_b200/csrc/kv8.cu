@@ -85,9 +85,15 @@ extern "C" int fg_kv8_expand(const void* k_pages, const void* v_pages, const flo
   return 0;
 }
 
-// Floats of scratch (the splits' partials) that fg_kv8_attention_decode needs for at most max_pairs (request, split) pairs.
-extern "C" long long fg_kv8_decode_scratch_floats(int n_heads, long long max_pairs) {
-  return max_pairs * n_heads * fg_mma::part_stride<FG_HEAD_DIM>();
+// What fg_kv8_attention_decode needs: floats of scratch, whatever the step, and zeroed counters, one for every sequence and
+// slice of up to eight heads of a group, which a launch leaves at zero.
+extern "C" int fg_kv8_decode_scratch_floats() {
+  using namespace fg_kv8;
+  return decode_blocks_per_sm<FG_HEAD_DIM>() * fg_sm_count() * 2 * MAX_COLUMNS * run_stride<FG_HEAD_DIM>();
+}
+extern "C" int fg_kv8_decode_counters(int n_seqs, int n_heads, int n_kv_heads) {
+  const int group = n_heads / n_kv_heads;
+  return n_seqs * n_kv_heads * ((group + fg_kv8::MAX_COLUMNS - 1) / fg_kv8::MAX_COLUMNS);
 }
 
 // Attention of single tokens; pools as tensor maps made by fg_make_kv8_tensor_map, `layer` the run's index in them.
@@ -95,19 +101,19 @@ extern "C" int fg_kv8_attention_decode(const void* q, int q_stride, void* out, i
                                        const void* v_map, int layer, const float* k_scales, const float* v_scales,
                                        const int* block_table, int table_width, int page_size, int n_pages, const int* pos,
                                        const int* seq_req, const int* seq_tok, int n_seqs, int n_heads, int n_kv_heads,
-                                       int head_dim, int window, float scale, float softcap, float* scratch,
-                                       long long scratch_floats, int max_splits, long long max_pairs, const float* out_freqs,
-                                       const float* sinks, int* status, cudaStream_t stream) {
+                                       int head_dim, int window, float scale, float softcap, float* scratch, int scratch_floats,
+                                       int* counters, int n_counters, const float* out_freqs, const float* sinks, int* status,
+                                       cudaStream_t stream) {
   using namespace fg_kv8;
   if (n_seqs == 0) return 0;
   if (check_pages("fg_kv8_attention_decode", q, out, k_scales, v_scales, page_size, n_pages, n_kv_heads, head_dim)) return -1;
-  FG_CHECK_ARG(n_heads > 0 && n_heads % n_kv_heads == 0 && n_heads <= 65535 && n_seqs <= DECODE_MAX_SEQS,
+  FG_CHECK_ARG(n_heads > 0 && n_heads % n_kv_heads == 0 && n_seqs <= DECODE_MAX_SEQS,
                "fg_kv8_attention_decode: %d heads over %d kv heads, %d sequences (at most %d)", n_heads, n_kv_heads, n_seqs,
                DECODE_MAX_SEQS);
-  FG_CHECK_ARG(max_splits > 0 && scratch != nullptr && max_pairs > 0 &&
-                   scratch_floats >= fg_kv8_decode_scratch_floats(n_heads, max_pairs),
-               "fg_kv8_attention_decode: scratch of %lld floats is too small", scratch_floats);
-  FG_CHECK_ARG(q_stride % 8 == 0, "fg_kv8_attention_decode: the queries' row stride must be a multiple of 8");
+  FG_CHECK_ARG(scratch != nullptr && scratch_floats >= fg_kv8_decode_scratch_floats() && counters != nullptr &&
+                   n_counters >= fg_kv8_decode_counters(n_seqs, n_heads, n_kv_heads) && ((uintptr_t)scratch & 15) == 0,
+               "fg_kv8_attention_decode: scratch of %d floats, %d counters are too few", scratch_floats, n_counters);
+  FG_CHECK_ARG(q_stride % 8 == 0 && out_stride % 2 == 0, "fg_kv8_attention_decode: row strides %d and %d", q_stride, out_stride);
   const int group = n_heads / n_kv_heads;
   CUtensorMap km, vm;
   memcpy(&km, k_map, sizeof(CUtensorMap));
@@ -120,19 +126,8 @@ extern "C" int fg_kv8_attention_decode(const void* q, int q_stride, void* out, i
   fg_launch_pdl(kern, dim3(decode_blocks_per_sm<FG_HEAD_DIM>() * fg_sm_count()), dim3(DECODE_THREADS), smem, stream, km, vm,
                 layer, k_scales, v_scales, (const __nv_bfloat16*)q, q_stride, block_table, table_width, page_size, n_pages, pos,
                 seq_req, seq_tok, n_seqs, n_heads, n_kv_heads, group, window, scale * log2e, softcap * log2e,
-                softcap > 0.f ? scale / softcap : 0.f, scratch, max_pairs, max_splits, status);
+                softcap > 0.f ? scale / softcap : 0.f, (__nv_bfloat16*)out, out_stride, scratch, counters, out_freqs, sinks,
+                status);
   FG_CHECK_LAUNCH("fg_kv8_attention_decode");
-  auto merge = [&](auto combine, int threads) {
-    fg_launch_pdl(combine, dim3(n_heads, n_seqs), dim3(threads), 0, stream, (const float*)scratch, (__nv_bfloat16*)out,
-                  out_stride, pos, seq_req, seq_tok, n_heads, window, max_splits, true, status, out_freqs, 0, sinks);
-  };
-  using namespace fg_mma;
-  constexpr int HALF = COMBINE_THREADS / 2;
-  // (as for the cache in 16 bits: half the threads a block where full blocks would be more than one round)
-  if ((long long)n_heads * n_seqs > 4ll * fg_sm_count())
-    merge(window < 0 ? attention_combine_kernel<FG_HEAD_DIM, true, HALF> : attention_combine_kernel<FG_HEAD_DIM, false, HALF>, HALF);
-  else
-    merge(window < 0 ? attention_combine_kernel<FG_HEAD_DIM, true> : attention_combine_kernel<FG_HEAD_DIM, false>, COMBINE_THREADS);
-  FG_CHECK_LAUNCH("fg_kv8_attention_decode (merge)");
   return 0;
 }

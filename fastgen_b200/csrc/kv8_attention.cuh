@@ -1,10 +1,15 @@
 // Attention of single tokens over the cache in 8 bits.
 //
-// Blocks stay on their SM and walk the (request, key/value head, split of 128 keys) items that exist, each block a stretch of
-// neighbours, so that a request's queries are converted once for many splits.  A producer warp streams codes through a ring
-// of shared-memory slots ahead of four consumer warps; partials per split go to scratch and attention_combine_kernel merges
-// them.  In the first product a consumer warp has 32 keys; the weights go to shared memory, and in the second product it
-// has a quarter of the dimensions of all 128 keys, so that there are no sums of warps to merge.
+// Blocks stay on their SM and walk the (request, key/value head, 128 keys) items that exist, each block a stretch of
+// neighbours, an equal share of all.  The items of one request and head inside a block are one run: queries converted once,
+// running maximum, sums and outputs in registers from item to item.  A run that holds all keys of its request is stored as the
+// result; the others leave a partial (two a block at most), and the block whose partial of a request and head is counted last
+// merges them in the order of the keys: one launch, nobody waits, the order of the sums is the walk's.  (A partial for
+// every 128 keys and a merge in a launch of its own: 64 ragged requests of up to 2,800 keys, 32 / 8 heads of 128, 62.6 us
+// against FIGURE_A, batch 8 at 4,096 keys 21.1 against FIGURE_B.)
+// A producer warp streams codes through a ring of shared-memory slots ahead of four consumer warps.  In the first product a
+// consumer warp has 32 keys; the weights go to shared memory, and in the second product it has a quarter of the dimensions
+// of all 128 keys, so that there are no sums of warps to merge.
 //
 //  * Codes become half precision on their way into a fragment, which is exact, by one conversion for two codes; bfloat16
 //    operands would need four instructions for two.  Queries are bfloat16, whose range half precision does not have: a
@@ -36,10 +41,9 @@ using fg_mma::mbar_arrive_expect;
 using fg_mma::mbar_fence_init;
 using fg_mma::mbar_init;
 using fg_mma::mbar_wait;
-using fg_mma::part_stride;
 using fg_mma::smem_u32;
 
-constexpr int SPLIT = fg_mma::DECODE_SPLIT;  // 128 key positions
+constexpr int SPLIT = 128;                   // key positions of an item
 constexpr int DECODE_THREADS = 160;          // 4 consumer warps + 1 producer warp
 constexpr int CONSUMERS = 128;
 constexpr int MAX_COLUMNS = 8;       // heads of a group that an item works on
@@ -51,6 +55,8 @@ template <int HD>
 __host__ __device__ constexpr int decode_slots() { return HD == 64 ? 6 : HD == 128 ? 4 : 3; }
 template <int HD>
 __host__ __device__ constexpr int decode_blocks_per_sm() { return HD <= 128 ? 3 : 2; }
+template <int HD>
+__host__ __device__ constexpr int run_stride() { return HD + 4; }  // a run's partial of one head: outputs, maximum, sum
 
 template <int HD>
 inline size_t decode_smem_bytes(int n_seqs) {
@@ -109,6 +115,30 @@ __device__ __forceinline__ int key_offset(int key, int piece) {
 template <int HD>
 __device__ __forceinline__ int value_offset(int group, int g, int i) { return swizzled(group * (HD / 32) + i, g); }
 
+// What outputs relative to the base-2 maximum `top` are multiplied by: one over the sum of the weights, of which the head's
+// sink (in natural units) is one more without a key.
+__device__ __forceinline__ float finish(float top, float sum, const float* sinks, int head) {
+  if (sinks == nullptr) return sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+  const float sink = sinks[head] * 1.4426950408889634f, m = fmaxf(top, sink);
+  const float f = top == -INFINITY ? 0.f : ex2(top - m);
+  return f / (sum * f + ex2(sink - m));
+}
+
+// Two neighbouring outputs, turned by position * frequency of their pair where a table is given.
+__device__ __noinline__ float2 turned_pair(float a, float b, float freq, int p) {
+  float sn, cs;
+  sincosf((float)p * freq, &sn, &cs);
+  return make_float2(a * cs - b * sn, b * cs + a * sn);
+}
+__device__ __forceinline__ void store_pair(__nv_bfloat16* dst, float a, float b, const float* freqs, int pair, int p) {
+  if (freqs != nullptr) {
+    const float2 v = turned_pair(a, b, freqs[pair], p);
+    a = v.x;
+    b = v.y;
+  }
+  *reinterpret_cast<__nv_bfloat162*>(dst) = __floats2bfloat162_rn(a, b);
+}
+
 template <int HD, bool CHUNKS>
 __global__ void __launch_bounds__(DECODE_THREADS, decode_blocks_per_sm<HD>())
 kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, int layer,
@@ -116,7 +146,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
                   const int* __restrict__ block_table, int table_width, int page_size, int n_pages,
                   const int* __restrict__ pos, const int* __restrict__ seq_req, const int* __restrict__ seq_tok, int n_seqs,
                   int n_heads, int n_kv_heads, int group, int window, float scale_log2, float cap_log2, float scale_by_cap,
-                  float* __restrict__ scratch, long long max_pairs, int max_splits, int* status) {
+                  __nv_bfloat16* out, int out_stride, float* scratch, int* counters, const float* __restrict__ out_freqs,
+                  const float* __restrict__ sinks, int* status) {
   constexpr int SLOTS = decode_slots<HD>();
   constexpr int SLOT_BYTES = SPLIT * HD;
   constexpr int KP = HD / 64;               // 16-byte pieces a lane loads of a key's row
@@ -131,7 +162,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
   __shared__ __align__(8) uint64_t full[SLOTS], empty[SLOTS];
   __shared__ int s_exp[SLOTS][2][TILES];     // exponents of the keys' and the values' boxes, with the keys' slot
   __shared__ __align__(8) uint2 s_weights[TILES][32];  // the second product's right operand
-  __shared__ float s_top[4][MAX_COLUMNS], s_sum[4][MAX_COLUMNS];
+  __shared__ __align__(8) float s_top[4][MAX_COLUMNS], s_sum[4][MAX_COLUMNS];
+  __shared__ int s_last;                     // whether this block's partial was counted last
   __shared__ int gave_up;                    // set by a wait that ran out (see mbar_wait)
 
   pdl_trigger();
@@ -146,7 +178,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
   }
   // positions, lists and block tables are inputs of the step: read while the kernel before this one finishes
   auto first_split = [&](int p) { return first_visible<CHUNKS>(p, window) / SPLIT; };
-  auto n_splits = [&](int p) { return p < 0 ? 0 : min(p / SPLIT, max_splits - 1) - first_split(p) + 1; };
+  auto n_splits = [&](int p) { return p < 0 ? 0 : p / SPLIT - first_split(p) + 1; };
   for (int sq = tid; sq < n_seqs; sq += DECODE_THREADS) s_pos[sq] = seq_req[sq] < 0 ? -1 : pos[seq_tok[sq]];
   __syncthreads();
   if (warp == 0) {
@@ -171,17 +203,15 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
 
   const int box_rows = min(page_size, SPLIT);
   const int n_boxes = SPLIT / box_rows, box_shift = 31 - __clz(box_rows), page_shift = 31 - __clz(page_size);
-  int n_pairs = s_cum[n_seqs];
-  if (n_pairs > max_pairs) {
-    // the scratch was sized for fewer: report instead of writing past it
-    if (tid == 0 && blockIdx.x == 0 && status) atomicOr(status, FG_STATUS_BAD_SPLITS);
-    n_pairs = 0;
-  }
   // items: request, then (key/value head, slice of up to eight heads of its group), then split
   const int n_sub = (group + MAX_COLUMNS - 1) / MAX_COLUMNS, slices = n_kv_heads * n_sub;
-  const long long total = (long long)n_pairs * slices;
-  const long long begin = total * blockIdx.x / gridDim.x;
-  const int count = (int)(total * (blockIdx.x + 1) / gridDim.x - begin);
+  const long long total = (long long)s_cum[n_seqs] * slices;
+  const int blocks = (int)min((long long)gridDim.x, total);  // that have items
+  auto begin_of = [&](int b) { return total * b / blocks; };
+  auto block_of = [&](long long item) { return (int)(((item + 1) * blocks - 1) / total); };
+  const bool busy = (int)blockIdx.x < blocks;
+  const long long begin = busy ? begin_of(blockIdx.x) : 0;
+  const int count = busy ? (int)(begin_of(blockIdx.x + 1) - begin) : 0;
   struct Walk {
     int seq, slice, split, n, p, first, k_begin;  // split counts from `first`, the request's first one; n of them
   };
@@ -283,12 +313,20 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     const int row_key = 4 * (g8 >> 1) + (g8 & 1);  // the key of row g8 of a tile; row g8 + 8 has that + 2
     Walk w = start();
     int slot = 0, use = 0;
-    bool fresh = true;
+    bool fresh = true;  // the item begins a run
     uint32_t qb[KP][4][2];
     float un[2] = {1.f, 1.f};  // what undoes the queries' scaling, of the two heads whose scores this thread gets
     int heads = 0, head0 = 0;
+    float run_top[2], run_sum[2];  // of heads 2 t4 and 2 t4 + 1; the sum over this thread's keys
+    float o[MINE][HALVES][4];
     for (int i = 0; i < count; ++i) {
       if (fresh) {
+        run_top[0] = run_top[1] = -INFINITY;
+        run_sum[0] = run_sum[1] = 0.f;
+#pragma unroll
+        for (int c = 0; c < MINE; ++c)
+#pragma unroll
+          for (int h = 0; h < HALVES; ++h) o[c][h][0] = o[c][h][1] = o[c][h][2] = o[c][h][3] = 0.f;
         const int g = w.slice / n_sub, sub = w.slice - g * n_sub;
         heads = min(MAX_COLUMNS, group - sub * MAX_COLUMNS);
         head0 = g * group + sub * MAX_COLUMNS;
@@ -329,7 +367,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
       }
       const int k0 = (w.first + w.split) * SPLIT;
       const bool edge = k0 < w.k_begin || k0 + SPLIT > w.p + 1;  // some keys of the split are not seen
-      const int last = w.p, k_begin = w.k_begin, pair = s_cum[w.seq] + w.split;
+      const int last = w.p, k_begin = w.k_begin;
 
       // S^T[keys, heads] = K Q^T for this warp's 32 keys
       const unsigned char* Ks = ring + slot * SLOT_BYTES;
@@ -363,7 +401,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
       }
 
       // this thread's scores: keys of row g8 and that + 2, heads 2 t4 and 2 t4 + 1
-      float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+      float top[2] = {run_top[0], run_top[1]};
       const float fe[2] = {(float)ev[0], (float)ev[1]};
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
@@ -386,10 +424,18 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
       if (g8 == 0) *reinterpret_cast<float2*>(&s_top[warp][2 * t4]) = make_float2(top[0], top[1]);
       asm volatile("bar.sync 1, %0;\n" ::"n"(CONSUMERS) : "memory");
 #pragma unroll
-      for (int o = 0; o < 4; ++o) {
-        const float2 other = *reinterpret_cast<const float2*>(&s_top[o][2 * t4]);
+      for (int x = 0; x < 4; ++x) {
+        const float2 other = *reinterpret_cast<const float2*>(&s_top[x][2 * t4]);
         top[0] = fmaxf(top[0], other.x);
         top[1] = fmaxf(top[1], other.y);
+      }
+      // what the run holds so far, relative to the new maximum
+      float keep[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        keep[h] = run_top[h] == -INFINITY ? 0.f : ex2(run_top[h] - top[h]);
+        run_top[h] = top[h];
+        run_sum[h] *= keep[h];
       }
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt)
@@ -397,7 +443,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
         for (int e = 0; e < 4; ++e) {
           const float m = top[e & 1];
           const float x = s[mt][e] == -INFINITY ? -INFINITY : s[mt][e] - m + WEIGHT_SHIFT;  // (m may be -inf: a NaN stays one)
-          sum[e & 1] += ex2(x);
+          run_sum[e & 1] += ex2(x);
           s[mt][e] = ex2(x + fe[mt]);
         }
       // the weights as the 8-column operand: an 8 x 8 transposition in registers for each half tile
@@ -405,21 +451,17 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
       for (int mt = 0; mt < 2; ++mt)
         s_weights[warp * 2 + mt][lane] =
             make_uint2(transposed_8x8(pack_f16(s[mt][0], s[mt][1])), transposed_8x8(pack_f16(s[mt][2], s[mt][3])));
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], o);
-      if (g8 == 0) *reinterpret_cast<float2*>(&s_sum[warp][2 * t4]) = make_float2(sum[0], sum[1]);
       asm volatile("bar.sync 1, %0;\n" ::"n"(CONSUMERS) : "memory");
 
       // O^T[dims, heads] = V^T P^T: this warp's pieces of all keys
       const unsigned char* Vs = ring + slot * SLOT_BYTES;
       mbar_wait(&full[slot], use & 1, status, &gave_up);
-      float o[MINE][HALVES][4];
 #pragma unroll
       for (int c = 0; c < MINE; ++c)
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h) o[c][h][0] = o[c][h][1] = o[c][h][2] = o[c][h][3] = 0.f;
+        for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[c][h][e] *= keep[e & 1];
 #pragma unroll
       for (int mt = 0; mt < TILES; ++mt) {
         const uint2 pb = s_weights[mt][lane];
@@ -455,33 +497,117 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
         ++use;
       }
 
-      float* part = scratch + ((size_t)pair * n_heads + head0) * part_stride<HD>();
+      const Walk at = w;
+      if (i + 1 < count) advance(w);
+      fresh = i + 1 == count || w.seq != at.seq || w.slice != at.slice;
+      if (!fresh) continue;
+
+      // ---- the run ends: the four warps' sums, then the result or a partial ----
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) run_sum[h] += __shfl_xor_sync(0xffffffffu, run_sum[h], x);
+      if (g8 == 0) *reinterpret_cast<float2*>(&s_sum[warp][2 * t4]) = make_float2(run_sum[0], run_sum[1]);
+      asm volatile("bar.sync 1, %0;\n" ::"n"(CONSUMERS) : "memory");
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float2 other = *reinterpret_cast<const float2*>(&s_sum[x][2 * t4]);
+        sum[0] += other.x;
+        sum[1] += other.y;
+      }
+      const long long run0 = (long long)s_cum[at.seq] * slices + (long long)at.slice * at.n;  // the request's first item of this head
+      __nv_bfloat16* const dst = out + (size_t)seq_tok[at.seq] * out_stride + head0 * HD;
+      if (run0 >= begin && run0 + at.n <= begin + count) {
+        // all keys of the request
+        float f[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int head = head0 + min(2 * t4 + e, heads - 1);
+          f[e] = finish(run_top[e] - WEIGHT_SHIFT, sum[e], sinks, head);
+        }
+#pragma unroll
+        for (int c = 0; c < MINE; ++c)
+#pragma unroll
+          for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              // rows g8 and g8 + 8 of the product are neighbouring dimensions
+              const int piece = HALVES == 2 ? warp + 4 * c : warp >> 1, which = HALVES == 2 ? h : warp & 1;
+              const int d = 4 * (g8 + 8 * piece) + 2 * which;
+              if (2 * t4 + e < heads)
+                store_pair(dst + (2 * t4 + e) * HD + d, o[c][h][e] * f[e], o[c][h][2 + e] * f[e], out_freqs, d / 2, at.p);
+            }
+        continue;
+      }
+      const int first_block = block_of(run0), last_block = block_of(run0 + at.n - 1);
+      // a block's partials: of the run that reaches back behind its stretch, and of the one that goes on after it
+      float* part = scratch + ((size_t)blockIdx.x * 2 + (run0 >= begin)) * MAX_COLUMNS * run_stride<HD>();
 #pragma unroll
       for (int c = 0; c < MINE; ++c)
 #pragma unroll
         for (int h = 0; h < HALVES; ++h)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            // rows g8 and g8 + 8 of the product are neighbouring dimensions
             const int piece = HALVES == 2 ? warp + 4 * c : warp >> 1, which = HALVES == 2 ? h : warp & 1;
             if (2 * t4 + e < heads)
-              *reinterpret_cast<float2*>(part + (2 * t4 + e) * part_stride<HD>() + 4 * (g8 + 8 * piece) + 2 * which) =
+              *reinterpret_cast<float2*>(part + (2 * t4 + e) * run_stride<HD>() + 4 * (g8 + 8 * piece) + 2 * which) =
                   make_float2(o[c][h][e], o[c][h][2 + e]);
           }
-      if (warp == 0 && g8 == 0) {
+      if (warp == 0 && g8 == 0)
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          if (2 * t4 + e < heads) {
-            float l = 0.f;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) l += s_sum[x][2 * t4 + e];
-            *reinterpret_cast<float2*>(part + (2 * t4 + e) * part_stride<HD>() + HD) = make_float2(top[e] - WEIGHT_SHIFT, l);
-          }
+          if (2 * t4 + e < heads)
+            *reinterpret_cast<float2*>(part + (2 * t4 + e) * run_stride<HD>() + HD) = make_float2(run_top[e] - WEIGHT_SHIFT, sum[e]);
+      __threadfence();
+      asm volatile("bar.sync 1, %0;\n" ::"n"(CONSUMERS) : "memory");
+      if (tid == 0) {
+        int* counter = counters + (size_t)at.seq * slices + at.slice;
+        const int last_one = atomicAdd(counter, 1) == last_block - first_block;
+        if (last_one) *counter = 0;  // for the launches behind this one
+        s_last = last_one;
+        __threadfence();
       }
-      if (i + 1 < count) {
-        const int seq = w.seq, slice = w.slice;
-        advance(w);
-        fresh = w.seq != seq || w.slice != slice;
+      asm volatile("bar.sync 1, %0;\n" ::"n"(CONSUMERS) : "memory");
+      if (!s_last) continue;
+      // every partial of this request and head is there: a thread merges four neighbouring dimensions of a head, eight
+      // partials' loads in flight together
+      for (int x = tid; x < heads * (HD / 4); x += CONSUMERS) {
+        const int r = x / (HD / 4), d = 4 * (x - r * (HD / 4));
+        float m = -INFINITY, l = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int b0 = first_block; b0 <= last_block; b0 += 8) {
+          float2 ml[8];
+          float4 v[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const int b = b0 + u;
+            const float* from = scratch + (((size_t)min(b, last_block) * 2 + (b == first_block)) * MAX_COLUMNS + r) * run_stride<HD>();
+            ml[u] = __ldcg(reinterpret_cast<const float2*>(from + HD));
+            v[u] = __ldcg(reinterpret_cast<const float4*>(from + d));
+            if (b > last_block) ml[u].x = -INFINITY;
+          }
+          float top = m;
+#pragma unroll
+          for (int u = 0; u < 8; ++u) top = fmaxf(top, ml[u].x);
+          const float keep = m == -INFINITY ? 0.f : ex2(m - top);
+          m = top;
+          l *= keep;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) a[e] *= keep;
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            if (b0 + u > last_block) break;
+            const float f = ml[u].x == -INFINITY ? 0.f : ex2(ml[u].x - top);
+            l += f * ml[u].y;
+            a[0] += f * v[u].x;
+            a[1] += f * v[u].y;
+            a[2] += f * v[u].z;
+            a[3] += f * v[u].w;
+          }
+        }
+        const float f = finish(m, l, sinks, head0 + r);
+        store_pair(dst + r * HD + d, a[0] * f, a[1] * f, out_freqs, d / 2, at.p);
+        store_pair(dst + r * HD + d + 2, a[2] * f, a[3] * f, out_freqs, d / 2 + 1, at.p);
       }
     }
   }

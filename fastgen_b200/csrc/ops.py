@@ -247,7 +247,9 @@ _KV8_SIGNATURES = {
     "fg_kv8_values": [_P, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _P, _P],
     "fg_kv8_expand": [_P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P],
     "fg_kv8_attention_decode": [_P, _I, _P, _I, _P, _P, _I, _P, _P, _P, _I, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _F, _F, _P,
-                                ctypes.c_longlong, _I, ctypes.c_longlong, _P, _P, _P, _P],
+                                _I, _P, _I, _P, _P, _P, _P],
+    "fg_kv8_decode_scratch_floats": [],
+    "fg_kv8_decode_counters": [_I, _I, _I],
 }
 _kv8 = {}
 _delta = None
@@ -320,8 +322,6 @@ def kv8(head_dim: int):
     if lib is None:
         lib = build.kv8_library(head_dim)
         _declare(lib, _KV8_SIGNATURES)
-        lib.fg_kv8_decode_scratch_floats.argtypes = [_I, ctypes.c_longlong]
-        lib.fg_kv8_decode_scratch_floats.restype = ctypes.c_longlong
         _kv8[head_dim] = lib
     return lib
 
@@ -411,6 +411,10 @@ class Ops:
         # (pages, kv heads, page, head size) of an 8-bit cache -> its pages in bfloat16 as prompt portions read
         # them (keys, values, tensor maps); every layer and group of these sizes fills the same pool in turn
         self._expanded = {}
+        # head size -> partials and counters of the single-token attention over a cache in 8 bits
+        self._kv8_buffers = {}
+        self._kv8_retired = []
+        self._kv8_stream = None  # whose work the two are used by
         self._latent_maps = {}  # (address, shape, box) of a layer's latent pool -> its tensor map
         self.use_tcgen05 = not bool(os.environ.get("FG_NO_TCGEN05"))
         # library products accumulate and reduce in float32 (no bfloat16 split-K sums)
@@ -427,6 +431,8 @@ class Ops:
             flags.zero_()
         for _scratch, flags in self._split_retired:
             flags.zero_()
+        for counters in [*self._kv8_retired, *(count for _scratch, count in self._kv8_buffers.values())]:
+            counters.zero_()
 
     def check_status(self) -> None:
         """Read the device status word (synchronises) and raise if a kernel
@@ -1678,6 +1684,7 @@ class Ops:
     def kv8_expanded(self, memory):
         """The pool that prompt portions over a cache of this shape read: keys and values in bfloat16 and their tensor
         maps.  Made at the first call (not inside a graph capture) and kept."""
+        self._one_stream()
         key = tuple(memory.k_pages.shape)
         got = self._expanded.get(key)
         if got is None:
@@ -1687,6 +1694,32 @@ class Ops:
             v = torch.zeros_like(k)
             got = self._expanded[key] = (k, v, self.make_kv_tensor_maps(k[None], v[None], key[2]))
         return got
+
+    def _one_stream(self) -> None:
+        """The work buffers of the cache in 8 bits belong to one stream at a time: a call on another stream than the last
+        one's is ordered behind what that one holds so far.  (Captured graphs of one :class:`Ops` are replayed one after
+        the other, as an engine does.)"""
+        stream = _stream()
+        if stream != self._kv8_stream and not torch.cuda.is_current_stream_capturing():
+            if self._kv8_stream is not None:
+                torch.cuda.current_stream(self.device).wait_stream(torch.cuda.ExternalStream(self._kv8_stream, self.device))
+            self._kv8_stream = stream
+
+    def _kv8_work(self, lib, head_dim: int, counters: int):
+        """Scratch and zeroed counters of the single-token attention over a cache in 8 bits.  They grow outside graph captures
+        only; buffers that were outgrown stay alive, since captured graphs may hold their addresses."""
+        self._one_stream()
+        scratch, count = self._kv8_buffers.get(head_dim, (None, None))
+        if scratch is None or count.numel() < counters:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the first single-token attention of a size over a cache in 8 bits cannot be inside a graph capture")
+            if scratch is None:
+                scratch = torch.empty(lib.fg_kv8_decode_scratch_floats(), dtype=torch.float32, device=self.device)
+            else:
+                self._kv8_retired.append(count)
+            count = torch.zeros(max(1024, 1 << (counters - 1).bit_length()), dtype=torch.int32, device=self.device)
+            self._kv8_buffers[head_dim] = (scratch, count)
+        return scratch, count
 
     def _attention_kv8(self, q, out, memory, ctx, n_heads, n_kv_heads, head_dim, window, scale, out_freqs, keep_first,
                        softcap, sinks, chunk) -> bool:
@@ -1714,16 +1747,13 @@ class Ops:
                            softcap=softcap, sinks=sinks, chunk=chunk)
         fused = out_freqs is not None and not prompts and singles.n > 0
         if singles.n:
-            max_splits = max(1, -(-singles.max_len // DECODE_SPLIT))
-            pairs = min(singles.n * max_splits, singles.stretches(DECODE_SPLIT))
-            scratch = self._decode_scratch(lib.fg_kv8_decode_scratch_floats(n_heads, pairs))
+            scratch, counters = self._kv8_work(lib, head_dim, lib.fg_kv8_decode_counters(singles.n, n_heads, n_kv_heads))
             _check(lib, lib.fg_kv8_attention_decode(
                 _ptr(q), q.stride(0), _ptr(out), out.stride(0), memory.tensor_maps[0].ptr, memory.tensor_maps[1].ptr,
                 memory.layer_index, _ptr(memory.k_scales), _ptr(memory.v_scales), _ptr(table), table.shape[1], page, n_pages,
                 _ptr(ctx.pos), _ptr(singles.req), _ptr(singles.tok), singles.n, n_heads, n_kv_heads, head_dim, signed_window,
-                float(scale), float(softcap or 0.0), _ptr(scratch), scratch.numel(), max_splits, pairs,
+                float(scale), float(softcap or 0.0), _ptr(scratch), scratch.numel(), _ptr(counters), counters.numel(),
                 _ptr(out_freqs) if fused else None, _ptr(sinks), _ptr(self.status), _stream()))
-            Ops.launches += 1  # the merge
         return fused
 
     def rotate_heads(self, x, pos, req, freqs, n_heads: int, head_dim: int) -> torch.Tensor:
