@@ -119,7 +119,8 @@ extern "C" int fg_kv8_attention_decode(const void* q, int q_stride, void* out, i
   memcpy(&km, k_map, sizeof(CUtensorMap));
   memcpy(&vm, v_map, sizeof(CUtensorMap));
   const size_t smem = decode_smem_bytes<FG_HEAD_DIM>(n_seqs);
-  auto kern = window < 0 ? kv8_decode_kernel<FG_HEAD_DIM, true> : kv8_decode_kernel<FG_HEAD_DIM, false>;
+  auto kern = window < 0 ? (softcap > 0.f ? kv8_decode_kernel<FG_HEAD_DIM, true, true> : kv8_decode_kernel<FG_HEAD_DIM, true, false>)
+                         : (softcap > 0.f ? kv8_decode_kernel<FG_HEAD_DIM, false, true> : kv8_decode_kernel<FG_HEAD_DIM, false, false>);
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   FG_CHECK_ARG(e == cudaSuccess, "fg_kv8_attention_decode: shared memory: %s", cudaGetErrorString(e));
   const float log2e = 1.4426950408889634f;

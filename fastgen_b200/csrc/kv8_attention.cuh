@@ -139,7 +139,7 @@ __device__ __forceinline__ void store_pair(__nv_bfloat16* dst, float a, float b,
   *reinterpret_cast<__nv_bfloat162*>(dst) = __floats2bfloat162_rn(a, b);
 }
 
-template <int HD, bool CHUNKS>
+template <int HD, bool CHUNKS, bool CAPPED>
 __global__ void __launch_bounds__(DECODE_THREADS, decode_blocks_per_sm<HD>())
 kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, int layer,
                   const float* k_scales, const float* v_scales, const __nv_bfloat16* q, int q_stride,
@@ -311,6 +311,17 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     pdl_wait();
     const int g8 = lane >> 2, t4 = lane & 3;
     const int row_key = 4 * (g8 >> 1) + (g8 & 1);  // the key of row g8 of a tile; row g8 + 8 has that + 2
+    // where this lane's pieces lie in a slot: a tile of 16 keys further on they lie 16 HD bytes further on, at the same place of
+    // the swizzle's pattern
+    int k_at[KP][2], v_at[MINE];
+#pragma unroll
+    for (int c = 0; c < KP; ++c) {
+      k_at[c][0] = key_offset<HD>(warp * 32 + row_key, key_piece<HD>(t4, c));
+      k_at[c][1] = key_offset<HD>(warp * 32 + row_key + 2, key_piece<HD>(t4, c));
+    }
+#pragma unroll
+    for (int c = 0; c < MINE; ++c)
+      v_at[c] = HALVES == 2 ? value_offset<HD>(t4, g8, warp + 4 * c) : value_offset<HD>(t4, g8, warp >> 1) + (warp & 1) * 8;
     Walk w = start();
     int slot = 0, use = 0;
     bool fresh = true;  // the item begins a run
@@ -380,12 +391,10 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
         ek[mt] = s_exp[slot][0][box];
         ev[mt] = s_exp[slot][1][box];
         s[mt][0] = s[mt][1] = s[mt][2] = s[mt][3] = 0.f;
-        const int key = warp * 32 + mt * 16 + row_key;
 #pragma unroll
         for (int c = 0; c < KP; ++c) {
-          const int piece = key_piece<HD>(t4, c);
-          const uint4 a = *reinterpret_cast<const uint4*>(Ks + key_offset<HD>(key, piece));
-          const uint4 b = *reinterpret_cast<const uint4*>(Ks + key_offset<HD>(key + 2, piece));
+          const uint4 a = *reinterpret_cast<const uint4*>(Ks + k_at[c][0] + mt * 16 * HD);
+          const uint4 b = *reinterpret_cast<const uint4*>(Ks + k_at[c][1] + mt * 16 * HD);
           const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
           for (int m = 0; m < 4; ++m)
@@ -401,22 +410,37 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
       }
 
       // this thread's scores: keys of row g8 and that + 2, heads 2 t4 and 2 t4 + 1
+      // s becomes the base-2 score plus the exponent of the value's scale
       float top[2] = {run_top[0], run_top[1]};
       const float fe[2] = {(float)ev[0], (float)ev[1]};
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
         const float ks = exp2_int(max(ek[mt], -126));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float sc = capped_score(s[mt][e] * un[e & 1] * ks, scale_log2, cap_log2, scale_by_cap);
-          if (edge || ek[mt] == NO_PAGE) {
-            const int j = k0 + warp * 32 + mt * 16 + row_key + (e & 2);
-            if (j < k_begin || j > last || ek[mt] == NO_PAGE) sc = -INFINITY;
+        for (int h = 0; h < 2; ++h) {
+          if constexpr (CAPPED) {
+            s[mt][h] = capped_score(s[mt][h] * ks * un[h], scale_log2, cap_log2, scale_by_cap) + fe[mt];
+            s[mt][2 + h] = capped_score(s[mt][2 + h] * ks * un[h], scale_log2, cap_log2, scale_by_cap) + fe[mt];
+          } else {
+            const float f = ks * (un[h] * scale_log2);
+            s[mt][h] = fmaf(s[mt][h], f, fe[mt]);
+            s[mt][2 + h] = fmaf(s[mt][2 + h], f, fe[mt]);
           }
-          s[mt][e] = sc;
-          top[e & 1] = fmaxf(top[e & 1], sc + fe[mt]);
         }
       }
+      if (edge || ek[0] == NO_PAGE || ek[1] == NO_PAGE) {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int j = k0 + warp * 32 + mt * 16 + row_key + (e & 2);
+            if (j < k_begin || j > last || ek[mt] == NO_PAGE) s[mt][e] = -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top[e & 1] = fmaxf(top[e & 1], s[mt][e]);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -437,15 +461,28 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
         run_top[h] = top[h];
         run_sum[h] *= keep[h];
       }
+      const float base[2] = {WEIGHT_SHIFT - (top[0] == -INFINITY ? 0.f : top[0]), WEIGHT_SHIFT - (top[1] == -INFINITY ? 0.f : top[1])};
+      // The softmax's own weight is the value's weight over its scale, 2^-f: a multiplication where the scales are near
+      // one another.  (A weight that is zero in float32 is 2^-141 of the largest: over scales up to 2^50 apart 2^-41.)
+      if (max(abs(ev[0]), abs(ev[1])) <= 50) {
+        const float inv[2] = {exp2_int(-ev[0]), exp2_int(-ev[1])};
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
+        for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float m = top[e & 1];
-          const float x = s[mt][e] == -INFINITY ? -INFINITY : s[mt][e] - m + WEIGHT_SHIFT;  // (m may be -inf: a NaN stays one)
-          run_sum[e & 1] += ex2(x);
-          s[mt][e] = ex2(x + fe[mt]);
-        }
+          for (int e = 0; e < 4; ++e) {
+            s[mt][e] = ex2(s[mt][e] + base[e & 1]);
+            run_sum[e & 1] = fmaf(s[mt][e], inv[mt], run_sum[e & 1]);
+          }
+      } else {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = s[mt][e] + base[e & 1];
+            s[mt][e] = ex2(x);
+            run_sum[e & 1] += ex2(x - fe[mt]);
+          }
+      }
       // the weights as the 8-column operand: an 8 x 8 transposition in registers for each half tile
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt)
@@ -479,12 +516,12 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
         for (int c = 0; c < MINE; ++c) {
           // dimensions 4 (g8 + 8 i) + 0..3 of the four keys of group t4 of the tile; at HD = 64 a warp has two of the four
           if constexpr (HALVES == 2) {
-            uint4 v = *reinterpret_cast<const uint4*>(Vs + value_offset<HD>(mt * 4 + t4, g8, warp + 4 * c));
+            uint4 v = *reinterpret_cast<const uint4*>(Vs + v_at[c] + mt * 16 * HD);
             if (edge) v.x &= mask, v.y &= mask, v.z &= mask, v.w &= mask;
             mma_f16(o[c][0], halves_of_low(v.x), halves_of_low(v.y), halves_of_high(v.x), halves_of_high(v.y), pb.x, pb.y);
             mma_f16(o[c][1], halves_of_low(v.z), halves_of_low(v.w), halves_of_high(v.z), halves_of_high(v.w), pb.x, pb.y);
           } else {
-            uint2 v = *reinterpret_cast<const uint2*>(Vs + value_offset<HD>(mt * 4 + t4, g8, warp >> 1) + (warp & 1) * 8);
+            uint2 v = *reinterpret_cast<const uint2*>(Vs + v_at[c] + mt * 16 * HD);
             if (edge) v.x &= mask, v.y &= mask;
             mma_f16(o[c][0], halves_of_low(v.x), halves_of_low(v.y), halves_of_high(v.x), halves_of_high(v.y), pb.x, pb.y);
           }

@@ -23,6 +23,9 @@ from . import build
 
 FG_F32, FG_BF16 = 0, 1
 
+_BF16, _F32, _E4M3 = torch.bfloat16, torch.float32, torch.float8_e4m3fn
+_KV8_PAGES = (16, 32, 64, 128, 256)  # tokens a page of a cache in 8 bits
+
 STATUS_BAD_PAGE = 1
 STATUS_BAD_TOKEN = 2
 STATUS_WAIT_TIMEOUT = 4
@@ -1146,27 +1149,31 @@ class Ops:
     def _linear4(self, x, w: Weight4, out=None, out_dtype=None, bias=None, act=None, gated: bool = False) -> torch.Tensor:
         """The product with 4-bit weights.  ``gated``: the rows of ``w`` are gate and up in blocks of 8 in turn, ``act`` a key of
         ``GATES``, and the result is the gated half."""
-        (m, k), (n, wk) = x.shape, w.shape
-        if self.act_dtype != torch.bfloat16 or x.dtype != torch.bfloat16:
+        m, k = x.shape
+        n = w.rows
+        if x.dtype is not _BF16 or self.act_dtype is not _BF16:
             raise ValueError(f"4-bit weights take bfloat16 activations, got {x.dtype}")
-        if wk != k or x.stride(1) != 1:
+        if w.columns != k or x.stride(1) != 1:
             raise ValueError(f"a product of {tuple(x.shape)} with 4-bit weights {w.shape}")
-        if bias is not None and (bias.shape != (n,) or bias.dtype != torch.bfloat16 or not bias.is_contiguous()):
+        if bias is not None and (bias.shape != (n,) or bias.dtype is not _BF16 or not bias.is_contiguous()):
             raise ValueError(f"the bias of {n} rows is contiguous bfloat16, got {bias.dtype} {tuple(bias.shape)}")
-        if x.stride(0) % 8 or x.data_ptr() % 16:
+        ldx, at = x.stride(0), x.data_ptr()
+        if ldx % 8 or at % 16:
             x = x.contiguous() if not x.is_contiguous() else x.clone()  # rows off 16 bytes (k is a multiple of 32)
+            ldx, at = x.stride(0), x.data_ptr()
         if out is None:
-            out = torch.empty((m, n // 2 if gated else n), dtype=out_dtype or torch.bfloat16, device=x.device)
-        assert out.stride(1) == 1 and tuple(out.shape) == (m, n // 2 if gated else n)
+            out = torch.empty((m, n // 2 if gated else n), dtype=out_dtype or _BF16, device=x.device)
+        else:
+            assert out.stride(1) == 1 and out.shape == (m, n // 2 if gated else n)
         code = GATES[act or "silu"] if gated else ACTIVATIONS[act]
         if m <= W4_MAX_M:
             _check(self.lib, self.lib.fg_gemm_w4(
-                _ptr(x), x.stride(0), _ptr(w.packed), _ptr(w.scales), w.group, _ptr(out), out.stride(0), _code(out.dtype),
-                m, n, k, _ptr(bias), code, int(gated), _stream()))
+                at, ldx, w.packed.data_ptr(), w.scales.data_ptr(), w.group, out.data_ptr(), out.stride(0), _code(out.dtype),
+                m, n, k, _ptr(bias), code, gated, _stream()))
         else:
             _check(self.lib, self.lib.fg_gemm_w4_tc5(
-                _ptr(x), x.stride(0), _ptr(w.packed), _ptr(w.scales), w.group, _ptr(out), out.stride(0), _code(out.dtype),
-                m, n, k, _ptr(bias), code, int(gated), 0, _ptr(self.status), _stream()))
+                at, ldx, w.packed.data_ptr(), w.scales.data_ptr(), w.group, out.data_ptr(), out.stride(0), _code(out.dtype),
+                m, n, k, _ptr(bias), code, gated, 0, self.status.data_ptr(), _stream()))
         return out
 
     def _skinny_ok(self, x: torch.Tensor, w: torch.Tensor, k: int) -> bool:
@@ -1592,25 +1599,31 @@ class Ops:
         """``None``, or why a cache of these sizes cannot be held in 8 bits."""
         if head_dim not in build.KV8_HEAD_DIMS:
             return f"head size {head_dim} is not one of {build.KV8_HEAD_DIMS}"
-        if not 16 <= page_size <= 256 or page_size & (page_size - 1):
+        if page_size not in _KV8_PAGES:
             return f"pages of {page_size} tokens are not a power of two from 16 to 256"
         return None
 
     def _check_kv8(self, memory, n_kv_heads: int, head_dim: int) -> None:
-        why = self.kv8_supported(head_dim, memory.page_size)
+        """Raise unless ``memory`` is a cache in 8 bits of these sizes."""
+        k, v, ks, vs, page = memory.k_pages, memory.v_pages, memory.k_scales, memory.v_scales, memory.page_size
+        n_pages = k.shape[0]
+        shape, scales = (n_pages, n_kv_heads, page, head_dim), (n_pages, n_kv_heads)
+        if (k.shape == shape and v.shape == (n_pages, n_kv_heads, page // 4, head_dim, 4) and ks.shape == scales == vs.shape
+                and k.dtype is v.dtype is _E4M3 and ks.dtype is vs.dtype is _F32 and k.is_contiguous() and v.is_contiguous()
+                and ks.is_contiguous() and vs.is_contiguous() and head_dim in build.KV8_HEAD_DIMS and page in _KV8_PAGES
+                and self.act_dtype is _BF16):
+            return
+        why = self.kv8_supported(head_dim, page)
         if why is not None:
             raise ValueError(f"a cache in 8 bits: {why}")
         if self.act_dtype != torch.bfloat16:
             raise ValueError("a cache in 8 bits serves bfloat16 models")
-        n_pages, page = memory.k_pages.shape[0], memory.page_size
-        for t, shape in ((memory.k_pages, (n_pages, n_kv_heads, page, head_dim)),
-                         (memory.v_pages, (n_pages, n_kv_heads, page // 4, head_dim, 4))):
-            if t.dtype != torch.float8_e4m3fn or tuple(t.shape) != shape or not t.is_contiguous():
-                raise ValueError(f"pages of a cache in 8 bits are contiguous e4m3 codes {shape}, got {t.dtype} {tuple(t.shape)}")
-        for t in (memory.k_scales, memory.v_scales):
-            if t.dtype != torch.float32 or tuple(t.shape) != (n_pages, n_kv_heads) or not t.is_contiguous():
-                raise ValueError(f"scales of a cache in 8 bits are contiguous float32 {(n_pages, n_kv_heads)}, "
-                                 f"got {t.dtype} {tuple(t.shape)}")
+        for t, dtype in ((k, _E4M3), (v, _E4M3), (ks, _F32), (vs, _F32)):
+            if t.dtype != dtype or not t.is_contiguous():
+                raise ValueError(f"a cache in 8 bits: contiguous {dtype} wanted, got {t.dtype} {tuple(t.shape)}")
+        raise ValueError(f"a cache in 8 bits of {n_kv_heads} heads of {head_dim}: keys {shape}, values "
+                         f"{(n_pages, n_kv_heads, page // 4, head_dim, 4)} and scales {scales} wanted, got {tuple(k.shape)}, "
+                         f"{tuple(v.shape)}, {tuple(ks.shape)} and {tuple(vs.shape)}")
 
     def make_kv8_tensor_maps(self, k_pool, v_pool):
         """Tensor maps of the pools of a cache in 8 bits: codes ``[layers, pages, kv heads, page, head size]`` of keys and
@@ -1640,31 +1653,31 @@ class Ops:
         Queries, keys and values are bfloat16; the rotated numbers are rounded once, to their codes."""
         self._check_kv8(memory, n_kv_heads, head_dim)
         t = q.shape[0]
-        for x, heads in ((q, n_heads), (k, n_kv_heads), (v, n_kv_heads)):
-            if x.dtype != torch.bfloat16 or x.stride(1) != 1 or tuple(x.shape) != (t, heads * head_dim):
-                raise ValueError(f"rope_kv8_write takes bfloat16 rows of {heads} heads of {head_dim}, got {x.dtype} {tuple(x.shape)}")
-        if n_heads % n_kv_heads:
-            raise ValueError(f"{n_heads} heads over {n_kv_heads} key/value heads")
-        assert pos.dtype == torch.int32 and req.dtype == torch.int32 and pos.numel() == req.numel() == t
+        kv_shape = (t, n_kv_heads * head_dim)
+        if not (q.shape == (t, n_heads * head_dim) and k.shape == kv_shape == v.shape and q.dtype is k.dtype is v.dtype is _BF16
+                and q.stride(1) == k.stride(1) == v.stride(1) == 1 and n_heads % n_kv_heads == 0):
+            raise ValueError(f"rope_kv8_write takes bfloat16 rows of {n_heads} and twice {n_kv_heads} heads of {head_dim}, got "
+                             f"{q.dtype} {tuple(q.shape)}, {k.dtype} {tuple(k.shape)} and {v.dtype} {tuple(v.shape)}")
         table = memory.block_table
-        assert table.dtype == torch.int32 and table.is_contiguous()
-        for f in (freqs, v_freqs):
-            assert f is None or (f.dtype == torch.float32 and f.numel() == head_dim // 2 and f.is_contiguous())
-        rstd, qn_w, kn_w = qk_norm if qk_norm is not None else (None, None, None)
+        assert pos.dtype is req.dtype is table.dtype is torch.int32 and pos.numel() == req.numel() == t and table.is_contiguous()
+        assert freqs is None or (freqs.dtype is _F32 and freqs.numel() == head_dim // 2 and freqs.is_contiguous())
+        assert v_freqs is None or (v_freqs.dtype is _F32 and v_freqs.numel() == head_dim // 2 and v_freqs.is_contiguous())
+        rstd = qn_w = kn_w = None
         rstd_heads = 0
-        if rstd is not None:
+        if qk_norm is not None:
+            rstd, qn_w, kn_w = qk_norm
             assert rstd.dtype == torch.float32 and rstd.is_contiguous() and rstd.shape[0] == t
             rstd_heads = 0 if rstd.shape[1] == 2 else rstd.shape[1]
             assert rstd_heads in (0, n_heads + n_kv_heads)
             assert qn_w is None or (qn_w.dtype == torch.float32 and qn_w.numel() == n_heads * head_dim and qn_w.is_contiguous())
             assert kn_w is None or (kn_w.dtype == torch.float32 and kn_w.numel() == n_kv_heads * head_dim and kn_w.is_contiguous())
-        out = torch.empty((t, n_heads * head_dim), dtype=torch.bfloat16, device=q.device)
+        out = torch.empty((t, n_heads * head_dim), dtype=_BF16, device=q.device)
         lib = kv8(head_dim)
         _check(lib, lib.fg_kv8_write(
-            _ptr(q), q.stride(0), _ptr(out), _ptr(k), k.stride(0), _ptr(v), v.stride(0), _ptr(pos), _ptr(req), _ptr(freqs),
-            _ptr(v_freqs), _ptr(memory.k_pages), _ptr(memory.v_pages), _ptr(memory.k_scales), _ptr(memory.v_scales),
-            _ptr(table), table.shape[1], memory.page_size, memory.k_pages.shape[0], t, n_heads, n_kv_heads, head_dim,
-            _ptr(self.status), _ptr(rstd), _ptr(qn_w), _ptr(kn_w), rstd_heads, float(magnitude), int(rot_pairs), _stream()))
+            q.data_ptr(), q.stride(0), out.data_ptr(), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), pos.data_ptr(),
+            req.data_ptr(), _ptr(freqs), _ptr(v_freqs), memory.k_pages.data_ptr(), memory.v_pages.data_ptr(),
+            memory.k_scales.data_ptr(), memory.v_scales.data_ptr(), table.data_ptr(), table.shape[1], memory.page_size,
+            memory.k_pages.shape[0], t, n_heads, n_kv_heads, head_dim, self.status.data_ptr(), _ptr(rstd), _ptr(qn_w), _ptr(kn_w), rstd_heads, float(magnitude), int(rot_pairs), _stream()))
         return out
 
     def kv8_values(self, memory, pages):
@@ -1672,13 +1685,14 @@ class Ops:
         ``[n, kv heads, page, head size]``, every slot of the pages, also those that hold no token."""
         n_pages, n_kv_heads, page, head_dim = memory.k_pages.shape
         self._check_kv8(memory, n_kv_heads, head_dim)
-        assert pages.dtype == torch.int32 and pages.is_contiguous()
-        k = torch.empty((pages.numel(), n_kv_heads, page, head_dim), dtype=torch.bfloat16, device=pages.device)
+        assert pages.dtype is torch.int32 and pages.is_contiguous()
+        n = pages.numel()
+        k = torch.empty((n, n_kv_heads, page, head_dim), dtype=_BF16, device=pages.device)
         v = torch.empty_like(k)
         lib = kv8(head_dim)
         _check(lib, lib.fg_kv8_values(
-            _ptr(memory.k_pages), _ptr(memory.v_pages), _ptr(memory.k_scales), _ptr(memory.v_scales), _ptr(pages), pages.numel(),
-            _ptr(k), _ptr(v), page, n_pages, n_kv_heads, head_dim, _ptr(self.status), _stream()))
+            memory.k_pages.data_ptr(), memory.v_pages.data_ptr(), memory.k_scales.data_ptr(), memory.v_scales.data_ptr(),
+            pages.data_ptr(), n, k.data_ptr(), v.data_ptr(), page, n_pages, n_kv_heads, head_dim, self.status.data_ptr(), _stream()))
         return k, v
 
     def kv8_expanded(self, memory):
@@ -1700,7 +1714,9 @@ class Ops:
         one's is ordered behind what that one holds so far.  (Captured graphs of one :class:`Ops` are replayed one after
         the other, as an engine does.)"""
         stream = _stream()
-        if stream != self._kv8_stream and not torch.cuda.is_current_stream_capturing():
+        if stream == self._kv8_stream:
+            return
+        if not torch.cuda.is_current_stream_capturing():
             if self._kv8_stream is not None:
                 torch.cuda.current_stream(self.device).wait_stream(torch.cuda.ExternalStream(self._kv8_stream, self.device))
             self._kv8_stream = stream
@@ -1724,9 +1740,9 @@ class Ops:
     def _attention_kv8(self, q, out, memory, ctx, n_heads, n_kv_heads, head_dim, window, scale, out_freqs, keep_first,
                        softcap, sinks, chunk) -> bool:
         self._check_kv8(memory, n_kv_heads, head_dim)
-        assert q.dtype == torch.bfloat16 and out.dtype == torch.bfloat16 and q.stride(1) == 1 and out.stride(1) == 1
+        assert q.dtype is out.dtype is _BF16 and q.stride(1) == 1 == out.stride(1)
         assert not (window and chunk)
-        assert sinks is None or (sinks.dtype == torch.float32 and sinks.numel() == n_heads and sinks.is_contiguous())
+        assert sinks is None or (sinks.dtype is _F32 and sinks.numel() == n_heads and sinks.is_contiguous())
         if window and keep_first:
             raise ValueError("a cache in 8 bits knows no window that keeps first positions")
         table = memory.block_table
@@ -1734,7 +1750,8 @@ class Ops:
         signed_window = -int(chunk) if chunk else int(window or 0)
         n_pages, page = memory.k_pages.shape[0], memory.page_size
         singles = ctx.single_tokens()
-        prompts = ctx.attention_tiles(attention_tiling(n_heads, n_kv_heads, PREFILL_TMA_ROWS), 2).n > 0
+        longest = getattr(ctx, "longest", None)
+        prompts = longest != 1 and ctx.attention_tiles(attention_tiling(n_heads, n_kv_heads, PREFILL_TMA_ROWS), 2).n > 0
         if prompts:
             k, v, maps = self.kv8_expanded(memory)
             _check(lib, lib.fg_kv8_expand(
@@ -1747,13 +1764,16 @@ class Ops:
                            softcap=softcap, sinks=sinks, chunk=chunk)
         fused = out_freqs is not None and not prompts and singles.n > 0
         if singles.n:
-            scratch, counters = self._kv8_work(lib, head_dim, lib.fg_kv8_decode_counters(singles.n, n_heads, n_kv_heads))
+            # a counter for every sequence and slice of up to eight heads of a group
+            slices = n_kv_heads * -(-n_heads // n_kv_heads // 8)
+            scratch, counters = self._kv8_work(lib, head_dim, singles.n * slices)
+            maps = memory.tensor_maps
             _check(lib, lib.fg_kv8_attention_decode(
-                _ptr(q), q.stride(0), _ptr(out), out.stride(0), memory.tensor_maps[0].ptr, memory.tensor_maps[1].ptr,
-                memory.layer_index, _ptr(memory.k_scales), _ptr(memory.v_scales), _ptr(table), table.shape[1], page, n_pages,
-                _ptr(ctx.pos), _ptr(singles.req), _ptr(singles.tok), singles.n, n_heads, n_kv_heads, head_dim, signed_window,
-                float(scale), float(softcap or 0.0), _ptr(scratch), scratch.numel(), _ptr(counters), counters.numel(),
-                _ptr(out_freqs) if fused else None, _ptr(sinks), _ptr(self.status), _stream()))
+                q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), maps[0].ptr, maps[1].ptr, memory.layer_index,
+                memory.k_scales.data_ptr(), memory.v_scales.data_ptr(), table.data_ptr(), table.shape[1], page, n_pages,
+                ctx.pos.data_ptr(), singles.req.data_ptr(), singles.tok.data_ptr(), singles.n, n_heads, n_kv_heads, head_dim,
+                signed_window, float(scale), float(softcap or 0.0), scratch.data_ptr(), scratch.numel(), counters.data_ptr(),
+                counters.numel(), _ptr(out_freqs) if fused else None, _ptr(sinks), self.status.data_ptr(), _stream()))
         return fused
 
     def rotate_heads(self, x, pos, req, freqs, n_heads: int, head_dim: int) -> torch.Tensor:

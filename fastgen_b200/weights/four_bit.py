@@ -33,6 +33,7 @@ class Weight4:
         self.packed = packed
         self.scales = scales
         self.group = group
+        self.rows, self.columns = packed.shape[0], 8 * packed.shape[1]
 
     @staticmethod
     def _packed(codes: torch.Tensor) -> torch.Tensor:
@@ -45,7 +46,7 @@ class Weight4:
 
     @property
     def shape(self) -> Tuple[int, int]:
-        return self.packed.shape[0], 8 * self.packed.shape[1]
+        return self.rows, self.columns
 
     @property
     def device(self) -> torch.device:
