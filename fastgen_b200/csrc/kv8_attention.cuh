@@ -163,13 +163,15 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
   __shared__ int s_exp[SLOTS][2][TILES];     // exponents of the keys' and the values' boxes, with the keys' slot
   __shared__ __align__(8) uint2 s_weights[TILES][32];  // the second product's right operand
   __shared__ __align__(8) float s_top[4][MAX_COLUMNS], s_sum[4][MAX_COLUMNS];
-  __shared__ int s_last;                     // whether this block's partial was counted last
+  __shared__ __align__(16) int s_run[2][4];                // the block's partials: request, slice, items of the run, position (-1: none)
+  __shared__ int s_last[2];                  // ... and whether this block's was counted last
   __shared__ int gave_up;                    // set by a wait that ran out (see mbar_wait)
 
   pdl_trigger();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) {
     gave_up = 0;
+    s_run[0][3] = s_run[1][3] = -1;
     for (int i = 0; i < SLOTS; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 4);  // one arrival a consumer warp
@@ -538,6 +540,14 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
       if (i + 1 < count) advance(w);
       fresh = i + 1 == count || w.seq != at.seq || w.slice != at.slice;
       if (!fresh) continue;
+      if (i + 1 < count && g8 < min(MAX_COLUMNS, group)) {
+        // the next run's queries on their way to L1
+        const int g = w.slice / n_sub, first = g * group + (w.slice - g * n_sub) * MAX_COLUMNS;
+        if (g8 < g * group + group - first) {
+          const __nv_bfloat16* row = q + (size_t)seq_tok[w.seq] * q_stride + (first + g8) * HD;
+          for (int c = t4; c < HD / 64; c += 4) asm volatile("prefetch.global.L1 [%0];\n" ::"l"(row + c * 64));
+        }
+      }
 
       // ---- the run ends: the four warps' sums, then the result or a partial ----
 #pragma unroll
@@ -577,9 +587,9 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
             }
         continue;
       }
-      const int first_block = block_of(run0), last_block = block_of(run0 + at.n - 1);
       // a block's partials: of the run that reaches back behind its stretch, and of the one that goes on after it
-      float* part = scratch + ((size_t)blockIdx.x * 2 + (run0 >= begin)) * MAX_COLUMNS * run_stride<HD>();
+      const int which_run = run0 >= begin;
+      float* part = scratch + ((size_t)blockIdx.x * 2 + which_run) * MAX_COLUMNS * run_stride<HD>();
 #pragma unroll
       for (int c = 0; c < MINE; ++c)
 #pragma unroll
@@ -596,21 +606,48 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
         for (int e = 0; e < 2; ++e)
           if (2 * t4 + e < heads)
             *reinterpret_cast<float2*>(part + (2 * t4 + e) * run_stride<HD>() + HD) = make_float2(run_top[e] - WEIGHT_SHIFT, sum[e]);
-      __threadfence();
-      asm volatile("bar.sync 1, %0;\n" ::"n"(CONSUMERS) : "memory");
-      if (tid == 0) {
-        int* counter = counters + (size_t)at.seq * slices + at.slice;
-        const int last_one = atomicAdd(counter, 1) == last_block - first_block;
-        if (last_one) *counter = 0;  // for the launches behind this one
-        s_last = last_one;
-        __threadfence();
+      if (tid == 0) *reinterpret_cast<int4*>(s_run[which_run]) = make_int4(at.seq, at.slice, at.n, at.p);
+    }
+
+    // ---- the block's partials are counted when all its items are done: fence and counters cost their latency once ----
+    asm volatile("bar.sync 1, %0;\n" ::"n"(CONSUMERS) : "memory");
+    if (s_run[0][3] < 0 && s_run[1][3] < 0) return;
+    auto blocks_of = [&](const int* run, int& first, int& last) {
+      const long long run0 = (long long)s_cum[run[0]] * slices + (long long)run[1] * run[2];
+      first = block_of(run0);
+      last = block_of(run0 + run[2] - 1);
+    };
+    if (tid == 0) {
+      __threadfence();  // (for the whole block: its stores are ordered before by the barrier)
+      int before[2] = {0, 0};
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        if (s_run[x][3] >= 0) before[x] = atomicAdd(counters + (size_t)s_run[x][0] * slices + s_run[x][1], 1);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        s_last[x] = 0;
+        if (s_run[x][3] < 0) continue;
+        int first_block, last_block;
+        blocks_of(s_run[x], first_block, last_block);
+        if (before[x] == last_block - first_block) {
+          counters[(size_t)s_run[x][0] * slices + s_run[x][1]] = 0;  // for the launches behind this one
+          s_last[x] = 1;
+        }
       }
-      asm volatile("bar.sync 1, %0;\n" ::"n"(CONSUMERS) : "memory");
-      if (!s_last) continue;
+      __threadfence();
+    }
+    asm volatile("bar.sync 1, %0;\n" ::"n"(CONSUMERS) : "memory");
+    for (int x = 0; x < 2; ++x) {
+      if (!s_last[x]) continue;
+      int first_block, last_block;
+      blocks_of(s_run[x], first_block, last_block);
+      const int g = s_run[x][1] / n_sub, sub = s_run[x][1] - g * n_sub, p = s_run[x][3];
+      const int heads = min(MAX_COLUMNS, group - sub * MAX_COLUMNS), head0 = g * group + sub * MAX_COLUMNS;
+      __nv_bfloat16* const dst = out + (size_t)seq_tok[s_run[x][0]] * out_stride + head0 * HD;
       // every partial of this request and head is there: a thread merges four neighbouring dimensions of a head, eight
       // partials' loads in flight together
-      for (int x = tid; x < heads * (HD / 4); x += CONSUMERS) {
-        const int r = x / (HD / 4), d = 4 * (x - r * (HD / 4));
+      for (int y = tid; y < heads * (HD / 4); y += CONSUMERS) {
+        const int r = y / (HD / 4), d = 4 * (y - r * (HD / 4));
         float m = -INFINITY, l = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
         for (int b0 = first_block; b0 <= last_block; b0 += 8) {
           float2 ml[8];
@@ -619,13 +656,19 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
           for (int u = 0; u < 8; ++u) {
             const int b = b0 + u;
             const float* from = scratch + (((size_t)min(b, last_block) * 2 + (b == first_block)) * MAX_COLUMNS + r) * run_stride<HD>();
-            ml[u] = __ldcg(reinterpret_cast<const float2*>(from + HD));
-            v[u] = __ldcg(reinterpret_cast<const float4*>(from + d));
-            if (b > last_block) ml[u].x = -INFINITY;
+            // (volatile: all sixteen leave before the first is waited for)
+            asm volatile("ld.global.cg.v2.f32 {%0,%1}, [%2];\n" : "=f"(ml[u].x), "=f"(ml[u].y) : "l"(from + HD) : "memory");
+            asm volatile("ld.global.cg.v4.f32 {%0,%1,%2,%3}, [%4];\n"
+                         : "=f"(v[u].x), "=f"(v[u].y), "=f"(v[u].z), "=f"(v[u].w)
+                         : "l"(from + d)
+                         : "memory");
           }
           float top = m;
 #pragma unroll
-          for (int u = 0; u < 8; ++u) top = fmaxf(top, ml[u].x);
+          for (int u = 0; u < 8; ++u) {
+            if (b0 + u > last_block) ml[u] = make_float2(-INFINITY, 0.f);  // (the last one once more: nothing)
+            top = fmaxf(top, ml[u].x);
+          }
           const float keep = m == -INFINITY ? 0.f : ex2(m - top);
           m = top;
           l *= keep;
@@ -633,7 +676,6 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
           for (int e = 0; e < 4; ++e) a[e] *= keep;
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
-            if (b0 + u > last_block) break;
             const float f = ml[u].x == -INFINITY ? 0.f : ex2(ml[u].x - top);
             l += f * ml[u].y;
             a[0] += f * v[u].x;
@@ -643,8 +685,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
           }
         }
         const float f = finish(m, l, sinks, head0 + r);
-        store_pair(dst + r * HD + d, a[0] * f, a[1] * f, out_freqs, d / 2, at.p);
-        store_pair(dst + r * HD + d + 2, a[2] * f, a[3] * f, out_freqs, d / 2 + 1, at.p);
+        store_pair(dst + r * HD + d, a[0] * f, a[1] * f, out_freqs, d / 2, p);
+        store_pair(dst + r * HD + d + 2, a[2] * f, a[3] * f, out_freqs, d / 2 + 1, p);
       }
     }
   }
