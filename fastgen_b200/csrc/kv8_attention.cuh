@@ -163,7 +163,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
   __shared__ int s_exp[SLOTS][2][TILES];     // exponents of the keys' and the values' boxes, with the keys' slot
   __shared__ __align__(8) uint2 s_weights[TILES][32];  // the second product's right operand
   __shared__ __align__(8) float s_top[4][MAX_COLUMNS], s_sum[4][MAX_COLUMNS];
-  __shared__ __align__(16) int s_run[2][4];                // the block's partials: request, slice, items of the run, position (-1: none)
+  __shared__ __align__(16) int s_run[2][8];  // the block's partials: request, slice, token, position (-1: none), blocks from and to
   __shared__ int s_last[2];                  // ... and whether this block's was counted last
   __shared__ int gave_up;                    // set by a wait that ran out (see mbar_wait)
 
@@ -209,8 +209,11 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
   const int n_sub = (group + MAX_COLUMNS - 1) / MAX_COLUMNS, slices = n_kv_heads * n_sub;
   const long long total = (long long)s_cum[n_seqs] * slices;
   const int blocks = (int)min((long long)gridDim.x, total);  // that have items
-  auto begin_of = [&](int b) { return total * b / blocks; };
-  auto block_of = [&](long long item) { return (int)(((item + 1) * blocks - 1) / total); };
+  // (64-bit divisions take a few hundred cycles; what is divided fits 32 bits up to some ten million items)
+  const bool narrow = (total + 1) * blocks < (1ll << 32);
+  auto divided = [&](long long a, long long b) { return narrow ? (long long)((uint32_t)a / (uint32_t)b) : a / b; };
+  auto begin_of = [&](int b) { return divided(total * b, blocks); };
+  auto block_of = [&](long long item) { return (int)divided((item + 1) * blocks - 1, total); };
   const bool busy = (int)blockIdx.x < blocks;
   const long long begin = busy ? begin_of(blockIdx.x) : 0;
   const int count = busy ? (int)(begin_of(blockIdx.x + 1) - begin) : 0;
@@ -329,7 +332,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     bool fresh = true;  // the item begins a run
     uint32_t qb[KP][4][2];
     float un[2] = {1.f, 1.f};  // what undoes the queries' scaling, of the two heads whose scores this thread gets
-    int heads = 0, head0 = 0;
+    int heads = 0, head0 = 0, tok = 0;
     float run_top[2], run_sum[2];  // of heads 2 t4 and 2 t4 + 1; the sum over this thread's keys
     float o[MINE][HALVES][4];
     for (int i = 0; i < count; ++i) {
@@ -344,7 +347,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
         heads = min(MAX_COLUMNS, group - sub * MAX_COLUMNS);
         head0 = g * group + sub * MAX_COLUMNS;
         // the queries as the 8-column operand: column lane / 4 is a head, its elements in the order of the keys' pieces
-        const __nv_bfloat16* row = q + (size_t)seq_tok[w.seq] * q_stride + (head0 + min(g8, heads - 1)) * HD;
+        tok = seq_tok[w.seq];
+        const __nv_bfloat16* row = q + (size_t)tok * q_stride + (head0 + min(g8, heads - 1)) * HD;
         uint4 raw[KP][2];
 #pragma unroll
         for (int c = 0; c < KP; ++c) {
@@ -564,7 +568,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
         sum[1] += other.y;
       }
       const long long run0 = (long long)s_cum[at.seq] * slices + (long long)at.slice * at.n;  // the request's first item of this head
-      __nv_bfloat16* const dst = out + (size_t)seq_tok[at.seq] * out_stride + head0 * HD;
+      __nv_bfloat16* const dst = out + (size_t)tok * out_stride + head0 * HD;
       if (run0 >= begin && run0 + at.n <= begin + count) {
         // all keys of the request
         float f[2];
@@ -606,44 +610,38 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
         for (int e = 0; e < 2; ++e)
           if (2 * t4 + e < heads)
             *reinterpret_cast<float2*>(part + (2 * t4 + e) * run_stride<HD>() + HD) = make_float2(run_top[e] - WEIGHT_SHIFT, sum[e]);
-      if (tid == 0) *reinterpret_cast<int4*>(s_run[which_run]) = make_int4(at.seq, at.slice, at.n, at.p);
+      if (tid == 0) {
+        *reinterpret_cast<int4*>(s_run[which_run]) = make_int4(at.seq, at.slice, tok, at.p);
+        s_run[which_run][4] = block_of(run0);
+        s_run[which_run][5] = block_of(run0 + at.n - 1);
+      }
     }
 
     // ---- the block's partials are counted when all its items are done: fence and counters cost their latency once ----
     asm volatile("bar.sync 1, %0;\n" ::"n"(CONSUMERS) : "memory");
     if (s_run[0][3] < 0 && s_run[1][3] < 0) return;
-    auto blocks_of = [&](const int* run, int& first, int& last) {
-      const long long run0 = (long long)s_cum[run[0]] * slices + (long long)run[1] * run[2];
-      first = block_of(run0);
-      last = block_of(run0 + run[2] - 1);
-    };
     if (tid == 0) {
-      __threadfence();  // (for the whole block: its stores are ordered before by the barrier)
-      int before[2] = {0, 0};
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-        if (s_run[x][3] >= 0) before[x] = atomicAdd(counters + (size_t)s_run[x][0] * slices + s_run[x][1], 1);
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         s_last[x] = 0;
         if (s_run[x][3] < 0) continue;
-        int first_block, last_block;
-        blocks_of(s_run[x], first_block, last_block);
-        if (before[x] == last_block - first_block) {
-          counters[(size_t)s_run[x][0] * slices + s_run[x][1]] = 0;  // for the launches behind this one
+        int* counter = counters + (size_t)s_run[x][0] * slices + s_run[x][1];
+        int before;
+        // (release for the whole block, whose stores are ordered before by the barrier; acquire for what the others stored)
+        asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;\n" : "=r"(before) : "l"(counter) : "memory");
+        if (before == s_run[x][5] - s_run[x][4]) {
+          *counter = 0;  // for the launches behind this one
           s_last[x] = 1;
         }
       }
-      __threadfence();
     }
     asm volatile("bar.sync 1, %0;\n" ::"n"(CONSUMERS) : "memory");
     for (int x = 0; x < 2; ++x) {
       if (!s_last[x]) continue;
-      int first_block, last_block;
-      blocks_of(s_run[x], first_block, last_block);
-      const int g = s_run[x][1] / n_sub, sub = s_run[x][1] - g * n_sub, p = s_run[x][3];
+      const int first_block = s_run[x][4], last_block = s_run[x][5], p = s_run[x][3];
+      const int g = s_run[x][1] / n_sub, sub = s_run[x][1] - g * n_sub;
       const int heads = min(MAX_COLUMNS, group - sub * MAX_COLUMNS), head0 = g * group + sub * MAX_COLUMNS;
-      __nv_bfloat16* const dst = out + (size_t)seq_tok[s_run[x][0]] * out_stride + head0 * HD;
+      __nv_bfloat16* const dst = out + (size_t)s_run[x][2] * out_stride + head0 * HD;
       // every partial of this request and head is there: a thread merges four neighbouring dimensions of a head, eight
       // partials' loads in flight together
       for (int y = tid; y < heads * (HD / 4); y += CONSUMERS) {
