@@ -8,19 +8,22 @@ namespace fg_kv8 {
 // ---------------------------------------------------------------------------------
 // The write.  A page's new tokens are a run: consecutive tokens of the step with the same request and page.  Its scale
 // needs the largest magnitude of the whole run (and the scale that the cached entries before it have), so a run is the
-// work of one block, found on the device: a block looks at STRETCH tokens, one a warp, and takes the runs that begin among
-// them, for one key/value head and keys or values.  A run of one token (a decoded token) is its warp's work; a longer run
-// is the block's, a warp for four slots at a time.  Blocks of the same stretch with higher indices rotate the queries.
+// work of one block, found on the device: a block looks at a stretch of tokens, PER a warp, and takes the runs that begin
+// among them, keys and values of one key/value head.  A run of one token (a decoded token) is a warp's work; a longer run is
+// the block's, a warp for four slots at a time, whose rows stay in registers between the search for the largest and the
+// rounding.  Blocks of the same stretch with higher indices rotate the queries.
+//
+// Bound by latencies: a block is a chain of positions, pages, rows, angles and codes.  Steps of many tokens take stretches
+// of 64 tokens (PER = 4), a page of the usual size: with 16, three of four blocks found no run and left (2,048 prompt
+// tokens beside 20 single ones, 32 / 8 heads of 128: 34 us with one token a warp, 18 now).
 // ---------------------------------------------------------------------------------
-constexpr int STRETCH = 16;
-constexpr int WRITE_THREADS = 32 * STRETCH;
-constexpr int Q_SLICE = 8;  // query heads a block rotates
+constexpr int WRITE_WARPS = 16, WRITE_THREADS = 32 * WRITE_WARPS;
+constexpr int Q_SLICE = 8, Q_FLIGHT = 8;  // query heads a block rotates, and those whose rows are in flight together
 
 // A lane's E = HD / 32 neighbouring elements of a row.
 template <int E, bool VEC>
-__device__ __forceinline__ void load_lane(float (&x)[E], const __nv_bfloat16* row, int lane) {
+__device__ __forceinline__ void load_lane(uint32_t (&w)[E / 2], const __nv_bfloat16* row, int lane) {
   const __nv_bfloat16* p = row + lane * E;
-  uint32_t w[E / 2];
   if constexpr (VEC) {
     if constexpr (E == 2) {
       w[0] = ld_global_4(p);
@@ -30,20 +33,26 @@ __device__ __forceinline__ void load_lane(float (&x)[E], const __nv_bfloat16* ro
       const uint4 v = ld_global_16(p);
       w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
     }
-#pragma unroll
-    for (int i = 0; i < E / 2; ++i) {
-      x[2 * i] = __uint_as_float(w[i] << 16);
-      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
   } else {
     const volatile unsigned short* s = reinterpret_cast<const volatile unsigned short*>(p);
 #pragma unroll
-    for (int i = 0; i < E; ++i) x[i] = __uint_as_float((uint32_t)s[i] << 16);
+    for (int i = 0; i < E / 2; ++i) {
+      const uint32_t lo = s[2 * i], hi = s[2 * i + 1];
+      w[i] = lo | (hi << 16);
+    }
+  }
+}
+template <int E>
+__device__ __forceinline__ void unpacked(float (&x)[E], const uint32_t (&w)[E / 2]) {
+#pragma unroll
+  for (int i = 0; i < E / 2; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
   }
 }
 
-template <int HD, bool VEC>
-__global__ void __launch_bounds__(WRITE_THREADS)
+template <int HD, bool VEC, int PER>
+__global__ void __launch_bounds__(WRITE_THREADS, HD <= 128 ? 2 : 1)
 kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, const __nv_bfloat16* k, int k_stride,
                  const __nv_bfloat16* v, int v_stride, const int* __restrict__ pos, const int* __restrict__ req,
                  const float* __restrict__ freqs, const float* __restrict__ v_freqs, unsigned char* k_pages,
@@ -51,14 +60,12 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
                  int page_size, int n_pages, int n_tokens, int n_heads, int n_kv_heads, int* status, const float* rstd,
                  const float* __restrict__ qn_w, const float* __restrict__ kn_w, int rstd_heads, float magnitude,
                  int rot_pairs) {
-  constexpr int E = HD / 32;
-  __shared__ int s_len[STRETCH], s_page[STRETCH];
-  __shared__ float s_amax[STRETCH];
+  constexpr int E = HD / 32, STRETCH = WRITE_WARPS * PER;
+  __shared__ int s_len[STRETCH], s_page[STRETCH], s_pos[STRETCH];
+  __shared__ float s_amax[2][WRITE_WARPS];
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int t0 = blockIdx.x * STRETCH, t = t0 + warp;
-  const int r = t < n_tokens ? req[t] : -1;
-  const int p = r >= 0 ? pos[t] : 0;
+  const int t0 = blockIdx.x * STRETCH;
   const int role = blockIdx.y;
 
   // sine and cosine of the lane's pairs at position p
@@ -85,7 +92,7 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
       x[2 * i + 1] = b * cs[i] + a * sn[i];
     }
   };
-  // the norm's factor of a token and head (column `at` of the factors, 0 or 1 where the whole projection shares one)
+  // the norm's factor of a token and head (column `at_head` of the factors, 0 or 1 where the whole projection shares one)
   auto normed = [&](float (&x)[E], int t, int at_head, int at_whole, const float* w) {
     if (rstd == nullptr) return;
     const float f = rstd_heads ? rstd[(size_t)t * rstd_heads + at_head] : rstd[2 * (size_t)t + at_whole];
@@ -93,85 +100,98 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
     for (int i = 0; i < E; ++i) x[i] *= f * (w ? w[lane * E + i] : 1.f);
   };
 
-  if (role >= 2 * n_kv_heads) {
+  if (role >= n_kv_heads) {
     // ---- queries: a warp a token, the heads of the slice ----
-    if (r < 0) return;
-    float sn[E / 2], cs[E / 2];
-    turns(sn, cs, freqs, p, magnitude);
-    pdl_wait();
-    const int h0 = (role - 2 * n_kv_heads) * Q_SLICE, h1 = min(n_heads, h0 + Q_SLICE);
-    float x[Q_SLICE][E];
+    const int h0 = (role - n_kv_heads) * Q_SLICE, h1 = min(n_heads, h0 + Q_SLICE);
+    bool waited = false;
+#pragma unroll 1
+    for (int u = 0; u < PER; ++u) {
+      const int t = t0 + warp * PER + u;
+      const int r = t < n_tokens ? req[t] : -1;
+      if (r < 0) continue;
+      float sn[E / 2], cs[E / 2];
+      turns(sn, cs, freqs, pos[t], magnitude);
+      if (!waited) pdl_wait();
+      waited = true;
+#pragma unroll 1
+      for (int hb = h0; hb < h1; hb += Q_FLIGHT) {
+        uint32_t raw[Q_FLIGHT][E / 2];
 #pragma unroll
-    for (int u = 0; u < Q_SLICE; ++u)
-      if (h0 + u < h1) load_lane<E, VEC>(x[u], q + (size_t)t * q_stride + (h0 + u) * HD, lane);
+        for (int i = 0; i < Q_FLIGHT; ++i)
+          if (hb + i < h1) load_lane<E, VEC>(raw[i], q + (size_t)t * q_stride + (hb + i) * HD, lane);
 #pragma unroll
-    for (int u = 0; u < Q_SLICE; ++u) {
-      const int h = h0 + u;
-      if (h >= h1) continue;
-      normed(x[u], t, h, 0, qn_w ? qn_w + h * HD : nullptr);
-      turn(x[u], sn, cs);
-      __nv_bfloat162 out[E / 2];
+        for (int i = 0; i < Q_FLIGHT; ++i) {
+          const int h = hb + i;
+          if (h >= h1) continue;
+          float x[E];
+          unpacked(x, raw[i]);
+          normed(x, t, h, 0, qn_w ? qn_w + h * HD : nullptr);
+          turn(x, sn, cs);
+          __nv_bfloat162 out[E / 2];
 #pragma unroll
-      for (int i = 0; i < E / 2; ++i) out[i] = __floats2bfloat162_rn(x[u][2 * i], x[u][2 * i + 1]);
-      __nv_bfloat16* dst = q_out + ((size_t)t * n_heads + h) * HD + lane * E;
-      if constexpr (VEC) {
-        if constexpr (E == 2) *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<uint32_t*>(out);
-        else if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(out);
-        else *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(out);
-      } else {
+          for (int e = 0; e < E / 2; ++e) out[e] = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
+          __nv_bfloat16* dst = q_out + ((size_t)t * n_heads + h) * HD + lane * E;
+          if constexpr (VEC) {
+            if constexpr (E == 2) *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<uint32_t*>(out);
+            else if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(out);
+            else *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(out);
+          } else {
 #pragma unroll
-        for (int i = 0; i < E / 2; ++i) dst[2 * i] = out[i].x, dst[2 * i + 1] = out[i].y;
+            for (int e = 0; e < E / 2; ++e) dst[2 * e] = out[e].x, dst[2 * e + 1] = out[e].y;
+          }
+        }
       }
     }
+    if (!waited) pdl_wait();
     return;
   }
 
-  // ---- keys or values of one head ----
-  const int g = role >> 1;
-  const bool is_v = role & 1;
-  const __nv_bfloat16* src = (is_v ? v : k) + g * HD;
-  const int src_stride = is_v ? v_stride : k_stride;
-  unsigned char* pool = is_v ? v_pages : k_pages;
-  float* scales = is_v ? v_scales : k_scales;
-  const float* table = is_v ? v_freqs : freqs;
-  const float mag = is_v ? 1.f : magnitude;
+  // ---- keys and values of one head ----
+  const int g = role;
+  const __nv_bfloat16* const src[2] = {k + g * HD, v + g * HD};
+  const int src_stride[2] = {k_stride, v_stride};
+  unsigned char* const pool[2] = {k_pages, v_pages};
+  float* const scales[2] = {k_scales, v_scales};
   const float* norm_w = kn_w ? kn_w + g * HD : nullptr;
 
-  // the run that begins at this warp's token: its length (0: none begins here) and its page
-  const int slot = p & (page_size - 1);
-  int len = 0, page = -1;
-  if (r >= 0 && (t == 0 || slot == 0 || req[t - 1] != r || pos[t - 1] != p - 1)) {
-    const int most = min(page_size - slot, n_tokens - t);
-    for (int at = 0; at < most; at += 32) {
-      const int i = at + lane;
-      const bool mine = i < most && req[t + i] == r && pos[t + i] == p + i;
-      const unsigned all = __ballot_sync(0xffffffffu, mine);
-      if (all != 0xffffffffu) {
-        len += __ffs(~all) - 1;
-        break;
+  // the runs that begin at this warp's tokens: their lengths (0: none begins there) and pages
+  bool any_long = false;
+#pragma unroll 1
+  for (int u = 0; u < PER; ++u) {
+    const int t = t0 + warp * PER + u;
+    const int r = t < n_tokens ? req[t] : -1;
+    const int p = r >= 0 ? pos[t] : 0;
+    const int slot = p & (page_size - 1);
+    int len = 0, page = -1;
+    if (r >= 0 && (t == 0 || slot == 0 || req[t - 1] != r || pos[t - 1] != p - 1)) {
+      const int logical = p / page_size;
+      page = logical < table_width ? block_table[(size_t)r * table_width + logical] : -1;
+      const int most = min(page_size - slot, n_tokens - t);
+      for (int at = 0; at < most; at += 32) {
+        const int i = at + lane;
+        const bool mine = i < most && req[t + i] == r && pos[t + i] == p + i;
+        const unsigned all = __ballot_sync(0xffffffffu, mine);
+        if (all != 0xffffffffu) {
+          len += __ffs(~all) - 1;
+          break;
+        }
+        len += 32;
       }
-      len += 32;
+      if (page < 0 || page >= n_pages) {
+        if (status && lane == 0) atomicOr(status, FG_STATUS_BAD_PAGE);
+        len = 0;
+      }
     }
-    const int logical = p / page_size;
-    page = logical < table_width ? block_table[(size_t)r * table_width + logical] : -1;
-    if (page < 0 || page >= n_pages) {
-      if (status && lane == 0) atomicOr(status, FG_STATUS_BAD_PAGE);
-      len = 0;
+    any_long = any_long || len > 1;
+    if (lane == 0) {
+      s_len[warp * PER + u] = len;
+      s_page[warp * PER + u] = page;
+      s_pos[warp * PER + u] = p;
     }
   }
-  if (lane == 0) {
-    s_len[warp] = len;
-    s_page[warp] = page;
-  }
-  float sn[E / 2], cs[E / 2];
-  if (len == 1) turns(sn, cs, table, p, mag);
-  __syncthreads();
+  any_long = __syncthreads_or(any_long);
   pdl_wait();
 
-  auto load_row = [&](float (&x)[E], int t) {
-    load_lane<E, VEC>(x, src + (size_t)t * src_stride, lane);
-    if (!is_v) normed(x, t, n_heads + g, 1, norm_w);
-  };
   auto row_amax = [&](const float (&x)[E]) {
     float a = 0.f;
 #pragma unroll
@@ -183,24 +203,24 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
   };
   auto over = [&](float x, float f) { return fabsf(x) <= 3.402823466e38f ? x * f : __int_as_float(0x7fffffff); };
   // the page's exponent: from the run's largest magnitude and, behind cached entries, no lower than theirs
-  auto exponents = [&](float amax, int slot, size_t block, int& old_e) {
+  auto exponents = [&](float amax, int slot, float before, int& old_e) {
     int e = scale_exponent(amax);
     old_e = e;
     if (slot > 0) {
-      old_e = exponent_of_scale(__uint_as_float(ld_global_4(scales + block)));
+      old_e = exponent_of_scale(before);
       e = max(e, old_e);
     }
     return e;
   };
   // cached entries before `slot` rounded again at a larger scale, by `n` threads of which this is number `i`
-  auto rescale = [&](size_t block, int slot, float f, int i, int n) {
-    unsigned char* base = pool + block * (size_t)page_size * HD;
-    const int whole = is_v ? (slot & ~3) * HD : slot * HD;  // bytes of whole rows (of whole groups of four rows)
+  auto rescale = [&](int kv, size_t block, int slot, float f, int i, int n) {
+    unsigned char* base = pool[kv] + block * (size_t)page_size * HD;
+    const int whole = kv ? (slot & ~3) * HD : slot * HD;  // bytes of whole rows (of whole groups of four rows)
     for (int at = i * 4; at < whole; at += n * 4) {
       uint32_t* w = reinterpret_cast<uint32_t*>(base + at);
       *w = rescaled(ld_global_4(w), f);
     }
-    if (is_v && (slot & 3)) {
+    if (kv && (slot & 3)) {
       const uint32_t mask = (1u << (8 * (slot & 3))) - 1u;  // tokens of the last group that are cached
       for (int d = i; d < HD; d += n) {
         uint32_t* w = reinterpret_cast<uint32_t*>(base + whole) + d;
@@ -210,12 +230,12 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
     }
   };
   // a lane's codes of one row
-  auto store_row = [&](const float (&x)[E], size_t block, int slot, float inv) {
-    unsigned char* base = pool + block * (size_t)page_size * HD;
+  auto store_row = [&](int kv, const float (&x)[E], size_t block, int slot, float inv) {
+    unsigned char* base = pool[kv] + block * (size_t)page_size * HD;
     uint32_t c[E / 2];
 #pragma unroll
     for (int i = 0; i < E / 2; ++i) c[i] = codes_of(over(x[2 * i], inv), over(x[2 * i + 1], inv));
-    if (!is_v) {
+    if (!kv) {
       unsigned char* dst = base + slot * HD + lane * E;
       if constexpr (E == 2) *reinterpret_cast<uint16_t*>(dst) = (uint16_t)c[0];
       else if constexpr (E == 4) *reinterpret_cast<uint32_t*>(dst) = c[0] | (c[1] << 16);
@@ -229,78 +249,126 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
       }
     }
   };
+  auto scale_before = [&](int kv, size_t block, int slot) {
+    return slot > 0 ? __uint_as_float(ld_global_4(scales[kv] + block)) : 1.f;
+  };
 
-  if (len == 1) {
-    float x[E];
-    load_row(x, t);
-    turn(x, sn, cs);
-    const float amax = warp_max(row_amax(x));
-    const size_t block = (size_t)page * n_kv_heads + g;
-    int old_e;
-    const int e = exponents(amax, slot, block, old_e);
-    if (e > old_e) {
-      rescale(block, slot, exp2_int(max(old_e - e, -126)), lane, 32);
-      __syncwarp();
+#pragma unroll 1
+  for (int u = 0; u < PER; ++u) {
+    if (s_len[warp * PER + u] != 1) continue;
+    const int t = t0 + warp * PER + u, p = s_pos[warp * PER + u], slot = p & (page_size - 1);
+    const size_t block = (size_t)s_page[warp * PER + u] * n_kv_heads + g;
+    uint32_t raw[2][E / 2];
+    load_lane<E, VEC>(raw[0], src[0] + (size_t)t * src_stride[0], lane);
+    load_lane<E, VEC>(raw[1], src[1] + (size_t)t * src_stride[1], lane);
+    const float before[2] = {scale_before(0, block, slot), scale_before(1, block, slot)};
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      float x[E];
+      unpacked(x, raw[kv]);
+      if (kv == 0) normed(x, t, n_heads + g, 1, norm_w);
+      if (kv == 0 || v_freqs != nullptr) {
+        float sn[E / 2], cs[E / 2];
+        turns(sn, cs, kv ? v_freqs : freqs, p, kv ? 1.f : magnitude);
+        turn(x, sn, cs);
+      }
+      const float amax = warp_max(row_amax(x));
+      int old_e;
+      const int e = exponents(amax, slot, before[kv], old_e);
+      if (e > old_e) {
+        rescale(kv, block, slot, exp2_int(max(old_e - e, -126)), lane, 32);
+        __syncwarp();
+      }
+      store_row(kv, x, block, slot, exp2_int(-e));
+      if (lane == 0 && (slot == 0 || e > old_e)) scales[kv][block] = exp2_int(e);
     }
-    store_row(x, block, slot, exp2_int(-e));
-    __syncwarp();  // every lane has read the old scale
-    if (lane == 0 && (slot == 0 || e > old_e)) scales[block] = exp2_int(e);
   }
+  if (!any_long) return;
 
+#pragma unroll 1
   for (int w = 0; w < STRETCH; ++w) {
     const int n = s_len[w];
     if (n <= 1) continue;
-    const int first = t0 + w, page = s_page[w];
-    const int p0 = pos[first], slot = p0 & (page_size - 1);
-    const size_t block = (size_t)page * n_kv_heads + g;
+    const int first = t0 + w, p0 = s_pos[w], slot = p0 & (page_size - 1);
+    const size_t block = (size_t)s_page[w] * n_kv_heads + g;
+    const float before[2] = {scale_before(0, block, slot), scale_before(1, block, slot)};
     // four slots a warp and round; pages of up to 64 slots need one round, whose rows stay in registers
-    const int rounds = (page_size + 4 * STRETCH - 1) / (4 * STRETCH);
-    float x[4][E];
-    auto load_round = [&](int c) {
-      const int s0 = 4 * (warp + STRETCH * c);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int s = s0 + i;
-#pragma unroll
-        for (int j = 0; j < E; ++j) x[i][j] = 0.f;
-        if (s >= slot && s < slot + n) load_row(x[i], first + s - slot);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int s = s0 + i;
-        if (table != nullptr && s >= slot && s < slot + n) {
-          float rs[E / 2], rc[E / 2];
-          turns(rs, rc, table, p0 + s - slot, mag);
-          turn(x[i], rs, rc);
-        }
+    const int rounds = (page_size + 4 * WRITE_WARPS - 1) / (4 * WRITE_WARPS);
+    uint32_t raw[2][4][E / 2];
+    float x[4][E];  // keys, turned
+    auto turned_v = [&](float (&y)[E], int i, int s) {
+      unpacked(y, raw[1][i]);
+      if (v_freqs != nullptr) {
+        float sn[E / 2], cs[E / 2];
+        turns(sn, cs, v_freqs, p0 + s - slot, 1.f);
+        turn(y, sn, cs);
       }
     };
-    float amax = 0.f;
+    auto load_round = [&](int c) {
+      const int s0 = 4 * (warp + WRITE_WARPS * c);
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int s = s0 + i;
+#pragma unroll
+          for (int j = 0; j < E / 2; ++j) raw[kv][i][j] = 0;
+          if (s >= slot && s < slot + n) load_lane<E, VEC>(raw[kv][i], src[kv] + (size_t)(first + s - slot) * src_stride[kv], lane);
+        }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int s = s0 + i;
+        unpacked(x[i], raw[0][i]);
+        if (s < slot || s >= slot + n) continue;
+        float sn[E / 2], cs[E / 2];
+        turns(sn, cs, freqs, p0 + s - slot, magnitude);
+        normed(x[i], first + s - slot, n_heads + g, 1, norm_w);
+        turn(x[i], sn, cs);
+      }
+    };
+    float amax[2] = {0.f, 0.f};
     for (int c = 0; c < rounds; ++c) {
       load_round(c);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) amax = fmaxf(amax, row_amax(x[i]));
+      for (int i = 0; i < 4; ++i) {
+        amax[0] = fmaxf(amax[0], row_amax(x[i]));
+        float y[E];
+        turned_v(y, i, 4 * (warp + WRITE_WARPS * c) + i);
+        amax[1] = fmaxf(amax[1], row_amax(y));
+      }
     }
-    amax = warp_max(amax);
+    amax[0] = warp_max(amax[0]);
+    amax[1] = warp_max(amax[1]);
     __syncthreads();  // the run before is through with s_amax
-    if (lane == 0) s_amax[warp] = amax;
+    if (lane == 0) {
+      s_amax[0][warp] = amax[0];
+      s_amax[1][warp] = amax[1];
+    }
     __syncthreads();
-    amax = warp_max(s_amax[lane & (STRETCH - 1)]);
-    int old_e;
-    const int e = exponents(amax, slot, block, old_e);
-    if (e > old_e) rescale(block, slot, exp2_int(max(old_e - e, -126)), threadIdx.x, WRITE_THREADS);
-    __syncthreads();  // rescaled entries share words with new ones; every thread has read the old scale
-    const float inv = exp2_int(-e);
+    int e[2], old_e[2];
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      amax[kv] = warp_max(s_amax[kv][lane & (WRITE_WARPS - 1)]);
+      e[kv] = exponents(amax[kv], slot, before[kv], old_e[kv]);
+      if (e[kv] > old_e[kv]) rescale(kv, block, slot, exp2_int(max(old_e[kv] - e[kv], -126)), threadIdx.x, WRITE_THREADS);
+    }
+    if (slot > 0) __syncthreads();  // rescaled entries share words with new ones; every thread has read the old scales
+    const float inv[2] = {exp2_int(-e[0]), exp2_int(-e[1])};
     for (int c = 0; c < rounds; ++c) {
       if (rounds > 1) load_round(c);
-      const int s0 = 4 * (warp + STRETCH * c);
-      if (is_v && s0 >= slot && s0 + 4 <= slot + n) {
+      const int s0 = 4 * (warp + WRITE_WARPS * c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (s0 + i >= slot && s0 + i < slot + n) store_row(0, x[i], block, s0 + i, inv[0]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) turned_v(x[i], i, s0 + i);  // now the values
+      if (s0 >= slot && s0 + 4 <= slot + n) {
         // a whole group of four tokens: words
-        uint32_t* dst = reinterpret_cast<uint32_t*>(pool + block * (size_t)page_size * HD + (size_t)s0 * HD) + lane * E;
+        uint32_t* dst = reinterpret_cast<uint32_t*>(v_pages + block * (size_t)page_size * HD + (size_t)s0 * HD) + lane * E;
         uint32_t wd[E];
 #pragma unroll
         for (int j = 0; j < E; ++j)
-          wd[j] = codes_of(over(x[0][j], inv), over(x[1][j], inv)) | (codes_of(over(x[2][j], inv), over(x[3][j], inv)) << 16);
+          wd[j] = codes_of(over(x[0][j], inv[1]), over(x[1][j], inv[1])) | (codes_of(over(x[2][j], inv[1]), over(x[3][j], inv[1])) << 16);
         if constexpr (E == 2) {
           *reinterpret_cast<uint2*>(dst) = make_uint2(wd[0], wd[1]);
         } else {
@@ -310,10 +378,14 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (s0 + i >= slot && s0 + i < slot + n) store_row(x[i], block, s0 + i, inv);
+          if (s0 + i >= slot && s0 + i < slot + n) store_row(1, x[i], block, s0 + i, inv[1]);
       }
     }
-    if (threadIdx.x == 0 && (slot == 0 || e > old_e)) scales[block] = exp2_int(e);
+    if (threadIdx.x < 2) {
+      const int kv = threadIdx.x;
+      const int mine = kv ? e[1] : e[0], old = kv ? old_e[1] : old_e[0];
+      if (slot == 0 || mine > old) scales[kv][block] = exp2_int(mine);
+    }
   }
 }
 
