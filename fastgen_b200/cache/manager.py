@@ -91,6 +91,8 @@ class CacheGroup:
     v_pages: Optional[torch.Tensor] = None  # the second pool; None when the spec asks for one
     device_table: Optional[torch.Tensor] = None  # [n_slots, table_width] int32
     tensor_maps: Optional[tuple] = None  # made by the kernels' side for pools it can tile
+    k_scales: Optional[torch.Tensor] = None  # a cache in 8 bits: [len(entries), n_pages, Hkv] float32, as v_scales
+    v_scales: Optional[torch.Tensor] = None
     dirty: List[Tuple[int, int, int]] = field(default_factory=list)  # (slot, col, page)
 
     def first_needed_page(self, length: int) -> int:
@@ -190,7 +192,14 @@ class CacheManager:
         tensor_map_factory=None,
         embedder_state: Optional[StateSpec] = None,
         table_writer=None,
+        cache_bits: int = 16,
     ) -> None:
+        """``cache_bits`` 8: keys and values are e4m3 codes with a scale for each page and head (see
+        :class:`LayerMemory`); ``dtype`` is then the type of the queries, and ``tensor_map_factory`` is given the two pools
+        only."""
+        if cache_bits not in (16, 8):
+            raise ValueError(f"a cache has 16 bits an entry (the compute type) or 8, got {cache_bits}")
+        self.cache_bits = cache_bits
         if page_size <= 0:
             raise ValueError(f"page size must be positive, got {page_size}")
         self.page_size = page_size
@@ -259,14 +268,25 @@ class CacheManager:
                     grp.page_size,
                     grp.spec.head_dim,
                 )
-                grp.k_pages = torch.zeros(shape, dtype=dtype, device=device)
-                if grp.spec.n_pools == 2:
-                    grp.v_pages = torch.zeros(shape, dtype=dtype, device=device)
+                if cache_bits == 8:
+                    if grp.spec.n_pools != 2 or grp.page_size % 4:
+                        raise ValueError("a cache in 8 bits holds keys and values in pages of a multiple of 4 tokens")
+                    runs, pages, heads, page, size = shape
+                    grp.k_pages = torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+                    grp.v_pages = torch.zeros((runs, pages, heads, page // 4, size, 4), dtype=torch.uint8,
+                                              device=device).view(torch.float8_e4m3fn)
+                    grp.k_scales = torch.ones((runs, pages, heads), dtype=torch.float32, device=device)
+                    grp.v_scales = torch.ones_like(grp.k_scales)
+                else:
+                    grp.k_pages = torch.zeros(shape, dtype=dtype, device=device)
+                    if grp.spec.n_pools == 2:
+                        grp.v_pages = torch.zeros(shape, dtype=dtype, device=device)
                 grp.device_table = torch.full(
                     (max_requests, grp.table_width), -1, dtype=torch.int32, device=device
                 )
                 if tensor_map_factory is not None and grp.v_pages is not None:
-                    grp.tensor_maps = tensor_map_factory(grp.k_pages, grp.v_pages, grp.page_size)
+                    pools = (grp.k_pages, grp.v_pages)
+                    grp.tensor_maps = tensor_map_factory(*pools) if cache_bits == 8 else tensor_map_factory(*pools, grp.page_size)
             for e, st in enumerate(self.state_specs):
                 if st is not None:
                     self.states[e] = torch.zeros(
@@ -433,6 +453,8 @@ class CacheManager:
             if grp.k_pages is not None:
                 mem.k_pages = grp.k_pages[i]
                 mem.v_pages = grp.v_pages[i] if grp.v_pages is not None else None
+                if grp.k_scales is not None:
+                    mem.k_scales, mem.v_scales = grp.k_scales[i], grp.v_scales[i]
                 mem.block_table = grp.device_table
                 mem.tensor_maps = grp.tensor_maps
                 mem.layer_index = i

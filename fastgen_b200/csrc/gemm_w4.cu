@@ -259,7 +259,41 @@ int by_group(int group, const void* x, int ldx, const void* w, const void* scale
   return choose<32, TO>(x, ldx, w, scales, y, ldy, M, N, K, epi, stream);
 }
 
+// The matrix in bfloat16, for products of many tokens: a thread eight columns.  Bound by its bytes: half of one read and two
+// written a weight (28,672 x 4,096: FIGURE_X).
+__global__ void __launch_bounds__(256)
+dense_kernel(const uint32_t* __restrict__ w, const __nv_bfloat16* __restrict__ scales, int group_words, uint4* out, size_t words) {
+  pdl_trigger();
+  pdl_wait();  // the memory written may still be read by the kernels before
+  const size_t step = (size_t)gridDim.x * blockDim.x;
+  for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < words; i += step) {
+    const uint32_t c = w[i];
+    const __nv_bfloat162 s = __bfloat162bfloat162(scales[i / group_words]);
+    uint32_t v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t x = weights_of(c, j);
+      const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x), s);
+      v[j] = *reinterpret_cast<const uint32_t*>(&y);
+    }
+    out[i] = make_uint4(v[0], v[1], v[2], v[3]);
+  }
+}
+
 }  // namespace
+
+// out: bf16 [N, K], each weight rounded once
+extern "C" int fg_w4_dense(const void* w, const void* scales, int group, void* out, int N, int K, cudaStream_t stream) {
+  FG_CHECK_ARG((group == 32 || group == 64 || group == 128) && N > 0 && K > 0 && K % group == 0, "fg_w4_dense: N=%d, K=%d in groups of %d",
+               N, K, group);
+  FG_CHECK_ARG(((uintptr_t)out & 15) == 0 && ((uintptr_t)w & 3) == 0, "fg_w4_dense: unaligned");
+  const size_t words = (size_t)N * (K / 8);
+  const size_t blocks = (words + 255) / 256, most = (size_t)16 * fg_sm_count();
+  fg_launch_pdl(dense_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, stream, (const uint32_t*)w,
+                (const __nv_bfloat16*)scales, group / 8, (uint4*)out, words);
+  FG_CHECK_LAUNCH("fg_w4_dense");
+  return 0;
+}
 
 extern "C" int fg_gemm_w4_max_m() { return 16; }
 

@@ -11,7 +11,7 @@
 
 Names and meanings of ``GenArgs``, ``Packet``, ``Fastgen.build/generate/destroy``
 follow fastgen/generate.py:30-76, 139-173, 405-425.  Options of the reference
-that belong to features outside this engine (host cache, fp8, tensor
+that belong to features outside this engine (host cache, tensor
 parallelism) are not present; ``tp_mesh`` must be ``None``.
 """
 
@@ -63,6 +63,10 @@ class GenArgs:
     sync_freq: int = 10
     seed: int = 777
 
+    cache_bits: int = 16  # 8: keys and values in 8 bits with a scale for each page and head (bfloat16 models)
+    weight_bits: int = 16  # 4: projections with 4-bit weights, a scale for each group of columns (bfloat16 models)
+    weight_group: int = 128  # columns of a group of 4-bit weights: 32, 64 or 128
+
 
 @dataclass
 class Packet:
@@ -98,8 +102,8 @@ class HfLoader:
     def has_tokenizer(self) -> bool:
         return (self.directory / "tokenizer.json").is_file()
 
-    def load(self, dtype: torch.dtype, device) -> Model:
-        return Model.load(self.directory, dtype, device)
+    def load(self, dtype: torch.dtype, device, weight_bits: int = 16, weight_group: int = 128) -> Model:
+        return Model.load(self.directory, dtype, device, weight_bits, weight_group)
 
 
 class Fastgen:
@@ -114,7 +118,10 @@ class Fastgen:
             raise ValueError("this engine runs on one GPU; tp_mesh must be None")
         device = torch.device(device)
         t0 = time.monotonic()
-        model = loader.load(dtype, device)
+        if gen_args.weight_bits == 16:
+            model = loader.load(dtype, device)
+        else:
+            model = loader.load(dtype, device, weight_bits=gen_args.weight_bits, weight_group=gen_args.weight_group)
         logger.info("Built and loaded model in %.2fs", time.monotonic() - t0)
         stop_tokens = list(model.args.stop_tokens)
         if loader.has_tokenizer():
@@ -141,7 +148,7 @@ class Fastgen:
         self._log_cuda_mem()
 
         # pages: from max_seq, or from the memory budget (generate.py:206-236)
-        per_token = model.cache_bytes_per_token(act_bytes)
+        per_token = model.cache_bytes_per_token(1 if args.cache_bits == 8 else act_bytes)
         widest = max((getattr(l.ffn.params, "ffn_dim", model.args.dim) if l.ffn is not None else model.args.dim
                       for l in model.args.layers))
         mp = mem_params(model.weight_bytes(), per_token, model.args.dim, widest, act_bytes,
@@ -165,7 +172,7 @@ class Fastgen:
         self.engine = Engine(
             model, page_size=block, n_pages=max_seq // block, max_requests=self.max_batch,
             max_length=min(model.args.max_positions, max_seq), num_cuda_graphs=args.num_cuda_graphs,
-            max_step_tokens=self.max_prefill,
+            max_step_tokens=self.max_prefill, cache_bits=args.cache_bits,
         )
         logger.info("Cache bytes per token: %d", per_token)
         logger.info("Allocated kv cache: %d pages of %d tokens", max_seq // block, block)

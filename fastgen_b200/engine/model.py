@@ -33,6 +33,7 @@ from ..parts.base import (
     split_pending,
 )
 from ..parts.params import TableEmbeddingParams
+from ..weights.four_bit import Weight4
 from ..weights.loader import load_weights
 
 
@@ -131,11 +132,16 @@ class Model:
         return [e.kv_from for e in self.args.schedule]
 
     def cache_bytes_per_token(self, elt_size: int) -> int:
-        """Bytes of keys and values one token adds over all runs that own a cache."""
+        """Bytes of keys and values one token adds over all runs that own a cache.  An element of one byte is a cache in 8
+        bits: prompt portions read such pages from a pool of one layer in the compute type, which is counted too."""
         total = 0
+        shapes = set()
         for spec, src in zip(self.cache_specs(), self.kv_from()):
             if spec is not None and src is None:
                 total += spec.n_pools * spec.n_kv_heads * spec.head_dim * elt_size
+                shapes.add((spec.n_kv_heads, spec.head_dim, spec.page_size))
+        if elt_size == 1:
+            total += sum(2 * heads * size * 2 for heads, size, _page in shapes)
         return total
 
     def weight_bytes(self) -> int:
@@ -151,6 +157,9 @@ class Model:
             for v in vars(part).values():
                 if isinstance(v, torch.Tensor):
                     add(v)
+                elif isinstance(v, Weight4):
+                    add(v.packed)
+                    add(v.scales)
                 elif isinstance(v, Part):  # a part made of parts (two mixers side by side)
                     add_part(v)
         add(self.output)
@@ -191,12 +200,15 @@ class Model:
             self.pass_embed = w[:, self.args.dim :].contiguous()
 
     @staticmethod
-    def load(model_dir, dtype: torch.dtype, device) -> "Model":
-        """Read ``config.json`` and the safetensors of ``model_dir``."""
-        from ..csrc.ops import Ops
+    def load(model_dir, dtype: torch.dtype, device, weight_bits: int = 16, weight_group: int = 128) -> "Model":
+        """Read ``config.json`` and the safetensors of ``model_dir``.  ``weight_bits`` 4: the projections of attention and
+        of dense feed-forwards become 4-bit weights as they are bound (groups of ``weight_group`` columns; bfloat16 only);
+        embeddings, the output matrix and other parts keep their type."""
+        from ..csrc.ops import Ops, check_weight_bits
 
+        check_weight_bits(dtype, weight_bits, weight_group)
         args = load_model_args(model_dir)
-        model = Model(args, Ops(dtype, device))
+        model = Model(args, Ops(dtype, device, weight_bits, weight_group))
         ignore = [args.output_name or "lm_head.weight"] if args.tie_embeddings else []
         ignore += list(args.optional_tensors)
         tensors = load_weights(model_dir, model.weight_specs(), device, ignore=ignore)
@@ -205,12 +217,13 @@ class Model:
         return model
 
     @staticmethod
-    def random(args: ModelArgs, dtype: torch.dtype, device, seed: int = 0) -> "Model":
+    def random(args: ModelArgs, dtype: torch.dtype, device, seed: int = 0, weight_bits: int = 16,
+               weight_group: int = 128) -> "Model":
         """A model with seeded random weights drawn on the device (no files):
         matrices N(0, 0.02), norm weights 1, as the random-weights writer does."""
         from ..csrc.ops import Ops
 
-        model = Model(args, Ops(dtype, device))
+        model = Model(args, Ops(dtype, device, weight_bits, weight_group))
         gen = torch.Generator(device=device).manual_seed(int(seed))
         tensors = {}
         for spec in model.weight_specs():

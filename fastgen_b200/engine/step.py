@@ -196,8 +196,12 @@ class Engine:
         num_cuda_graphs: int = 16,
         use_graphs: Optional[bool] = None,
         max_step_tokens: Optional[int] = None,
+        cache_bits: int = 16,
     ) -> None:
-        """``max_step_tokens``: steps of up to that many tokens that are not single tokens only
+        """``cache_bits`` 8: keys and values are held in 8 bits (e4m3 with a scale for each page and head) instead of the
+        compute type; for bfloat16 models whose mixers all take that, ``ValueError`` for others.
+
+        ``max_step_tokens``: steps of up to that many tokens that are not single tokens only
         (prompt portions, alone or beside decoded tokens) replay CUDA graphs too, captured per
         padded shape when first met (``engine/step_graph.py``); ``None``: such steps are launched
         kernel by kernel."""
@@ -209,6 +213,8 @@ class Engine:
             max_length = args.max_positions
         max_length = min(max_length, args.max_positions)
         self.max_length = max_length
+        if cache_bits == 8:
+            self._check_8_bits(model, page_size)
         self.cache = CacheManager(
             model.cache_specs(),
             model.state_specs(),
@@ -219,11 +225,16 @@ class Engine:
             max_length=max_length,
             dtype=model.ops.act_dtype,
             device=self.device,
-            tensor_map_factory=model.ops.make_kv_tensor_maps,
+            tensor_map_factory=model.ops.make_kv8_tensor_maps if cache_bits == 8 else model.ops.make_kv_tensor_maps,
             embedder_state=model.embedder_state_spec(),
             table_writer=model.ops.set_table_entries,
+            cache_bits=cache_bits,
         )
         self.memories = self.cache.memories()
+        if cache_bits == 8:
+            for mem in self.memories:
+                if mem.k_scales is not None:
+                    self.ops.kv8_expanded(mem)  # the pool that prompt portions read: now, not in the middle of a step
         self.last_h2d_bytes = 0
         if use_graphs is None:
             use_graphs = not bool(os.environ.get("FG_NO_CUDA_GRAPHS"))
@@ -235,6 +246,18 @@ class Engine:
             from .step_graph import StepGraphs
 
             self.step_graphs = StepGraphs(self, self.graphs, max_step_tokens)
+
+    @staticmethod
+    def _check_8_bits(model: Model, page_size: int) -> None:
+        if model.ops.act_dtype != torch.bfloat16:
+            raise ValueError("a cache in 8 bits serves bfloat16 models")
+        for block in model.blocks:
+            spec = block.mixer.cache_spec()
+            if spec is None:
+                continue
+            why = block.mixer.why_not_8_bits() or model.ops.kv8_supported(spec.head_dim, spec.page_size or page_size)
+            if why is not None:
+                raise ValueError(f"this model's cache cannot be held in 8 bits: {why}")
 
     # -- requests --------------------------------------------------------------
     def admit(self, request_id) -> RequestCache:

@@ -6,7 +6,8 @@ from typing import List, Optional
 
 import torch
 
-from .base import CacheSpec, Mixer, StateSpec, WeightSpec, make_position, register_mixer
+from ..weights.four_bit import Weight4
+from .base import CacheSpec, Mixer, StateSpec, WeightSpec, make_position, projection, register_mixer
 from .params import AttentionParams, SigmoidAttentionParams
 
 
@@ -137,6 +138,11 @@ class GQAAttention(Mixer):
         p = self.params
         return CacheSpec(p.n_kv_heads, self.hd, p.window, keep_first=p.keep_first if p.window else 0, chunk=p.chunk)
 
+    def why_not_8_bits(self) -> Optional[str]:
+        if self.params.window and self.params.keep_first:
+            return "attention whose window keeps a sequence's first positions reads a cache in the compute type only"
+        return None
+
     def state_spec(self) -> Optional[StateSpec]:
         p = self.params
         if not p.conv:
@@ -178,10 +184,10 @@ class GQAAttention(Mixer):
             wg = tensors["wg"].new_zeros((self.gate_rows, p.dim))
             wg[: p.n_heads] = tensors["wg"]
             parts.append(wg)
-        self.wqkv = torch.cat(parts, dim=0).to(dt).contiguous()
+        self.wqkv = projection(torch.cat(parts, dim=0), ops)
         # the output projection's columns follow the value heads' rows
         wo_t = self._rows(tensors["wo"].t(), p.n_heads, vd, p.v_layout, self.value_position)
-        self.wo = wo_t.t().to(dt).contiguous()
+        self.wo = projection(wo_t.t(), ops)
         self.bqkv = self.bo = None
         if p.bias:
             bq = self._rows(tensors["bq"], p.n_heads, p.head_dim, p.qk_layout, qk_pos)
@@ -236,7 +242,7 @@ class GQAAttention(Mixer):
         t = x.shape[0]
         q = None
         gate = None
-        if memory.writes and x.dtype == torch.bfloat16 and self.plain:
+        if memory.writes and x.dtype == torch.bfloat16 and self.plain and memory.k_scales is None and not isinstance(self.wqkv, Weight4):
             # a few tokens: projection, rotation and page write in one kernel
             q = ops.qkv_rope_write(x, self.wqkv, ctx.pos, ctx.req, self.freqs, memory,
                                    p.n_heads, p.n_kv_heads, self.hd, bias=self.bqkv, v_freqs=self.v_freqs)
@@ -272,11 +278,15 @@ class GQAAttention(Mixer):
                 # that rotates multiplies by them and by the weights
                 rstd = ops.qk_rstd(q, k, p.n_heads * p.head_dim, p.n_kv_heads * p.head_dim, p.qk_norm_eps, ctx.req)
                 qk_norm = (rstd, self.q_norm, self.k_norm)
-            ops.rope_kv_write(
-                q, k, v, ctx.pos, ctx.req, self.freqs, memory.k_pages, memory.v_pages,
-                memory.block_table, memory.page_size, p.n_heads, p.n_kv_heads, self.hd, v_freqs=self.v_freqs,
-                qk_norm=qk_norm, magnitude=self.magnitude, rot_pairs=self.rot_pairs,
-            )
+            if memory.writes and memory.k_scales is not None:
+                q = ops.rope_kv8_write(q, k, v, ctx.pos, ctx.req, self.freqs, memory, p.n_heads, p.n_kv_heads, self.hd,
+                                       v_freqs=self.v_freqs, qk_norm=qk_norm, magnitude=self.magnitude, rot_pairs=self.rot_pairs)
+            else:
+                ops.rope_kv_write(
+                    q, k, v, ctx.pos, ctx.req, self.freqs, memory.k_pages, memory.v_pages,
+                    memory.block_table, memory.page_size, p.n_heads, p.n_kv_heads, self.hd, v_freqs=self.v_freqs,
+                    qk_norm=qk_norm, magnitude=self.magnitude, rot_pairs=self.rot_pairs,
+                )
         o = torch.empty((t, self.q_width), dtype=x.dtype, device=x.device)
         turned = self._attend(q, o, ctx, memory)
         if self.v_unfreqs is not None and not turned:
@@ -294,6 +304,9 @@ class SigmoidAttention(GQAAttention):
     those of :class:`GQAAttention`; the per-head numbers are the tensors ``gate``, ``r1``, ``r2``."""
 
     params: SigmoidAttentionParams
+
+    def why_not_8_bits(self) -> Optional[str]:
+        return "attention with sigmoid weights reads a cache in the compute type only"
 
     def weight_specs(self) -> List[WeightSpec]:
         p = self.params

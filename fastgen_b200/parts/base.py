@@ -73,6 +73,16 @@ class StateSpec:
     dtype: torch.dtype = torch.float32
 
 
+def projection(w: torch.Tensor, ops):
+    """A projection's matrix [N, K] as ``ops.linear`` takes it: in the compute type, or as 4-bit weights where ``ops`` was
+    made for them."""
+    if getattr(ops, "weight_bits", 16) == 4:
+        from ..weights.four_bit import Weight4  # (that package's loader reads this module)
+
+        return Weight4.quantize(w, ops.weight_group)
+    return w.to(ops.act_dtype).contiguous()
+
+
 class Part:
     """Common base: weights are declared, then bound once they are on device."""
 
@@ -262,6 +272,11 @@ class Mixer(Part):
 
     def state_spec(self) -> Optional[StateSpec]:
         return None
+
+    def why_not_8_bits(self) -> Optional[str]:
+        """``None`` if the mixer's per-token entries may be held in 8 bits (its memory then comes with scales), or why
+        not.  Asked of mixers that cache."""
+        return f"{type(self).__name__} keeps its entries in the compute type"
 
     def forward(self, x: torch.Tensor, ctx, memory) -> torch.Tensor:
         """Mix tokens.  ``x`` is [T, dim] (normed), ``ctx`` the step's

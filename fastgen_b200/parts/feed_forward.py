@@ -6,7 +6,7 @@ from typing import List
 
 import torch
 
-from .base import FeedForward, WeightSpec, register_feed_forward
+from .base import FeedForward, WeightSpec, projection, register_feed_forward
 from .params import DenseMLPParams, SwiGLUParams
 
 
@@ -27,7 +27,6 @@ class SwiGLU(FeedForward):
 
     def bind(self, tensors, ops) -> None:
         self.ops = ops
-        dt = ops.act_dtype
         w1, w3 = tensors["w1"], tensors["w3"]
         f, d = w1.shape
         # gate and up rows interleaved in blocks of 8, so that 16 consecutive rows of
@@ -38,8 +37,8 @@ class SwiGLU(FeedForward):
             w13 = torch.stack([w1.view(f // 8, 8, d), w3.view(f // 8, 8, d)], dim=1).reshape(2 * f, d)
         else:
             w13 = torch.cat([w1, w3], dim=0)
-        self.w13 = w13.to(dt).contiguous()
-        self.w2 = tensors["w2"].to(dt).contiguous()
+        self.w13 = projection(w13, ops)
+        self.w2 = projection(tensors["w2"], ops)
 
     def forward(self, x, ctx):
         ops = self.ops
@@ -69,9 +68,8 @@ class DenseMLP(FeedForward):
 
     def bind(self, tensors, ops) -> None:
         self.ops = ops
-        dt = ops.act_dtype
-        self.up = tensors["up"].to(dt).contiguous()
-        self.down = tensors["down"].to(dt).contiguous()
+        self.up = projection(tensors["up"], ops)
+        self.down = projection(tensors["down"], ops)
 
     def forward(self, x, ctx):
         ops = self.ops

@@ -45,6 +45,9 @@ class SideBySide(Mixer):
     def cache_spec(self) -> Optional[CacheSpec]:
         return self.left.cache_spec() or self.right.cache_spec()
 
+    def why_not_8_bits(self) -> Optional[str]:
+        return (self.left if self.left.cache_spec() is not None else self.right).why_not_8_bits()
+
     def state_spec(self) -> Optional[StateSpec]:
         return self.left.state_spec() or self.right.state_spec()
 

@@ -39,6 +39,8 @@ def build_parser() -> argparse.ArgumentParser:
     parser.add_argument("--gpu-gb", type=float, default=20, help="approximate amount of gpu memory to use")
     parser.add_argument("--dtype", choices=["bf16", "fp32"], default="bf16", help="compute dtype")
     parser.add_argument("--page-size", type=int, default=64, help="tokens per cache page")
+    parser.add_argument("--cache-bits", type=int, choices=[16, 8], default=16, help="bits of a cached number")
+    parser.add_argument("--weight-bits", type=int, choices=[16, 4], default=16, help="bits of the projections' weights")
     parser.add_argument("--seed", type=int, default=777, help="seed of the sampler")
     parser.add_argument("--random-weights", metavar="CONFIG", help="write MODEL from this config.json first")
     parser.add_argument("--max-seq", type=int, default=-1, help="cache size in tokens (default: from --gpu-gb)")
@@ -73,6 +75,8 @@ def main(argv=None) -> int:
         cache_block=args.page_size,
         seed=args.seed,
         max_seq=args.max_seq,
+        cache_bits=args.cache_bits,
+        weight_bits=args.weight_bits,
     )
     dtype = torch.bfloat16 if args.dtype == "bf16" else torch.float32
     fg = Fastgen.build(loader, gen_args, tp_mesh=None, device=torch.device("cuda:0"), dtype=dtype)

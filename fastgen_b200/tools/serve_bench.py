@@ -131,6 +131,8 @@ def main() -> int:
     ap.add_argument("--max-prefill", type=int, default=0, help="tokens a step (0: the workload's own)")
     ap.add_argument("--sync-freq", type=int, default=10)
     ap.add_argument("--page", type=int, default=64)
+    ap.add_argument("--cache-bits", type=int, choices=[16, 8], default=16)
+    ap.add_argument("--weight-bits", type=int, choices=[16, 4], default=16)
     ap.add_argument("--graphs", type=int, default=32, help="most decode graphs (batch buckets)")
     ap.add_argument("--arrive-over", type=float, default=None,
                     help="seconds over which the requests arrive (0: all at once; default: the workload's own)")
@@ -145,14 +147,14 @@ def main() -> int:
     cfg = config_of(args.shape, args.layers)
     dev = torch.device("cuda:0")
     torch.cuda.set_device(dev)
-    model = Model.random(model_args_from_config(cfg), torch.bfloat16, dev, seed=w["seed"])
+    model = Model.random(model_args_from_config(cfg), torch.bfloat16, dev, seed=w["seed"], weight_bits=args.weight_bits)
     reqs = make_requests(args.shape, args.requests)
     max_batch = args.max_batch or len(reqs)
     longest = sorted((len(p) + g for p, g in reqs), reverse=True)[:max_batch]
     max_seq = sum(-(-(n + 1) // args.page) * args.page for n in longest) + 2 * args.page
     gen_args = GenArgs(use_sampling=False, max_batch=max_batch, max_seq=max_seq, cache_block=args.page,
                        max_prefill=args.max_prefill or w["max_prefill"], num_cuda_graphs=min(max_batch, args.graphs),
-                       sync_freq=args.sync_freq)
+                       sync_freq=args.sync_freq, cache_bits=args.cache_bits, weight_bits=args.weight_bits)
     fg = Fastgen(gen_args, model, stop_tokens=[])
 
     span = w["arrive_over"] if args.arrive_over is None else args.arrive_over
@@ -191,7 +193,7 @@ def main() -> int:
     first_seconds, _, _ = run(reqs)
     steps0, pre0, log0 = fg.steps, fg.scheduler.n_preemptions, len(fg.step_log)
     seconds, n_out, errors = run(reqs)
-    roofline = roofline_of(fg.step_log[log0:], cfg, model.weight_bytes(), model.cache_bytes_per_token(2),
+    roofline = roofline_of(fg.step_log[log0:], cfg, model.weight_bytes(), model.cache_bytes_per_token(args.cache_bits // 8),
                            gen_args.max_prefill, peaks())
     n_prompt = sum(len(p) for p, _ in reqs)
     line = {

@@ -98,7 +98,7 @@ class Weight4:
         packed, scales = [], []
         rows = max(1, (1 << 26) // k)
         for r in range(0, n, rows):
-            part = w[r : r + rows].float().view(-1, k // group, group)
+            part = w[r : r + rows].float().reshape(-1, k // group, group)
             s = (part.abs().amax(2) / 7.0).to(torch.bfloat16)
             # (a scale below bfloat16's range is zero, as if the group were)
             c = torch.round(torch.where(s.float().unsqueeze(2) > 0, part / s.float().unsqueeze(2), torch.zeros_like(part)))
