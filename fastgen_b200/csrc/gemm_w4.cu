@@ -1,6 +1,6 @@
 // Matrix product of a few tokens with 4-bit weights:
 //   y[M, N] = x[M, K] * W[N, K]^T,   W[n, k] = (code[n, k] - 8) * scale[n, k / G],   G = 32, 64 or 128,
-// x bfloat16, float32 accumulation, M <= 16.  (gemm_w4_tc5.cu has more tokens.)
+// x bfloat16, float32 accumulation, M <= 8.  (gemm_w4_tc5.cu has more tokens.)
 //
 // Bound by reading the codes once, half a byte a weight.  As in gemm_skinny.cu, 16 rows of W are the "M" side of
 // mma.sync m16n8k16 and 8 tokens its "N" side, a thread streams its own pieces through a ring of cp.async stages that only it
@@ -20,6 +20,7 @@ namespace {
 using namespace fg_skinny;
 
 constexpr int KCHUNK = 128;  // columns a warp takes at a time
+constexpr int TOKENS = 8;
 
 __device__ __forceinline__ void cp_async_4(void* dst, const void* src, bool pred) {
   const int bytes = pred ? 4 : 0;
@@ -35,15 +36,16 @@ __device__ __forceinline__ uint32_t weights_of(uint32_t w, int i) {
   return *reinterpret_cast<const uint32_t*>(&d);
 }
 
-// RT tiles of 16 rows and NT tiles of 8 tokens a block; G columns a group
-template <int RT_, int NT_, int G_>
+// RT tiles of 16 rows at a time a block; G columns a group
+template <int RT_, int G_>
 struct Plan4 {
-  static constexpr int RT = RT_, NT = NT_, G = G_;
-  static constexpr int PIECES = 2 * RT + 4 * NT;  // 16-byte pieces a thread copies per chunk
+  static constexpr int RT = RT_, G = G_;
+  static constexpr int PIECES = 2 * RT + 4;  // 16-byte pieces a thread copies per chunk: codes, x
   static constexpr int STAGES = PIECES <= 6 ? 4 : PIECES <= 8 ? 3 : 2;
   static constexpr size_t RING = (size_t)STAGES * PIECES * THREADS * 16;
-  static constexpr size_t SUMS = (size_t)WARPS * RT * ROWS * NT * 8 * 4;  // in the ring's memory once it is through
-  static constexpr size_t SMEM = RING > SUMS ? RING : SUMS;
+  static constexpr size_t SUMS = (size_t)WARPS * RT * ROWS * TOKENS * 4;
+  static constexpr size_t SMEM = RING + SUMS;
+  static constexpr int BLOCKS = SMEM <= 75 * 1024 ? 3 : 2;  // an SM
 };
 
 struct Epilogue4 {
@@ -52,180 +54,191 @@ struct Epilogue4 {
   bool gated;                 // rows are gate and up in blocks of 8: y[M, N / 2]
 };
 
+// A block works on a stretch of neighbouring tiles of 16 rows, an equal share of all, RT at a time; the copies of the next
+// ones run while the sums of the last are stored.
 template <typename P, typename TO>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, P::BLOCKS)
 gemm_w4_kernel(const __nv_bfloat16* x, int ldx, const uint32_t* __restrict__ w, int ldw, const __nv_bfloat16* __restrict__ scales,
                int lds, TO* __restrict__ y, int ldy, int M, int N, int K, Epilogue4 epi) {
-  constexpr int RT = P::RT, NT = P::NT, PARTS = KCHUNK / P::G;  // groups of a chunk
+  constexpr int RT = P::RT, PARTS = KCHUNK / P::G;  // groups of a chunk
+  // Rows beyond N and tokens beyond M are read as the last ones and left out of the result; K is whole chunks where the
+  // groups are (WHOLE), else columns beyond K are zeros.
+  constexpr bool WHOLE = P::G == KCHUNK;
+  constexpr int STEP = WARPS * KCHUNK;  // columns from one of the warp's chunks to its next
   extern __shared__ __align__(16) unsigned char ring_raw[];
-  uint4* ring = reinterpret_cast<uint4*>(ring_raw);  // [STAGES][PIECES][THREADS]
+  uint4* const ring = reinterpret_cast<uint4*>(ring_raw) + threadIdx.x;  // [STAGES][PIECES][THREADS]
+  typedef float Sums[RT * ROWS][TOKENS];
+  Sums* const red = reinterpret_cast<Sums*>(ring_raw + P::RING);  // [WARPS]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int n0 = blockIdx.x * (RT * ROWS);
+  const int tiles = (N + ROWS - 1) / ROWS;
+  const int first = (int)((long long)tiles * blockIdx.x / gridDim.x), last = (int)((long long)tiles * (blockIdx.x + 1) / gridDim.x);
   const int n_chunks = (K + KCHUNK - 1) / KCHUNK;
-  const int mine = warp < n_chunks ? (n_chunks - warp + WARPS - 1) / WARPS : 0;
+  const int mine = warp < n_chunks ? (n_chunks - warp + WARPS - 1) / WARPS : 0;  // of this warp, of every tile
   pdl_trigger();
 
-  auto issue_w = [&](int i) {
-    uint4* slot = ring + (size_t)(i % P::STAGES) * P::PIECES * THREADS + tid;
-    const int k = (warp + i * WARPS) * KCHUNK;
+  // the copies' place: tile, this warp's chunk of it, stage
+  int at_tile = first, at_chunk = 0, at_stage = 0;
+  uint32_t w_row[2 * RT];
+  auto rows_of = [&](int tile) {
+#pragma unroll
+    for (int r = 0; r < 2 * RT; ++r)
+      w_row[r] = (uint32_t)min(tile * ROWS + r * 8 + g, N - 1) * ldw + warp * (KCHUNK / 8) + (WHOLE ? 4 * t : t);
+  };
+  rows_of(first);
+  const uint32_t x_row = (uint32_t)min(g, M - 1) * ldx + warp * KCHUNK + (WHOLE ? 32 * t : 8 * t);
+  auto issue_w = [&](int tile, int i, uint4* slot) {
 #pragma unroll
     for (int r = 0; r < 2 * RT; ++r) {
-      const int n = n0 + r * 8 + g;
-      const uint32_t* row = w + (size_t)min(n, N - 1) * ldw;
-      if (P::G == KCHUNK) {
-        const int at = k + 32 * t;
-        cp_async_16<false>(slot + r * THREADS, row + (at < K ? at / 8 : 0), n < N && at < K);
+      if (r >= 2 && tile + r / 2 >= last) break;  // (the stretch's last tiles may be fewer than RT)
+      if (WHOLE) {
+        cp_async_16<false>(slot + r * THREADS, w + (w_row[r] + i * (STEP / 8)), true);
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int at = k + 32 * j + 8 * t;
-          cp_async_4(reinterpret_cast<uint32_t*>(slot + r * THREADS) + j, row + (at < K ? at / 8 : 0), n < N && at < K);
+          const bool ok = (warp + i * WARPS) * KCHUNK + 32 * j + 8 * t < K;
+          cp_async_4(reinterpret_cast<uint32_t*>(slot + r * THREADS) + j, w + (ok ? w_row[r] + i * (STEP / 8) + 4 * j : 0u), ok);
         }
       }
     }
   };
-  auto issue_x = [&](int i) {
-    uint4* slot = ring + (size_t)(i % P::STAGES) * P::PIECES * THREADS + tid;
-    const int k = (warp + i * WARPS) * KCHUNK;
+  auto issue_x = [&](int i, uint4* slot) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int tok = nt * 8 + g;
-      const __nv_bfloat16* row = x + (size_t)min(tok, M - 1) * ldx;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int at = k + (P::G == KCHUNK ? 32 * t + 8 * j : 32 * j + 8 * t);
-        cp_async_16<true>(slot + (2 * RT + nt * 4 + j) * THREADS, row + (at < K ? at : 0), tok < M && at < K);
-      }
+    for (int j = 0; j < 4; ++j) {
+      const bool ok = WHOLE || (warp + i * WARPS) * KCHUNK + 32 * j + 8 * t < K;
+      cp_async_16<true>(slot + (2 * RT + j) * THREADS, x + (ok ? x_row + i * STEP + (WHOLE ? 8 * j : 32 * j) : 0u), ok);
     }
   };
-  // the scales of a chunk: rows g + 8 r of the block, its groups
-  auto fetch_scales = [&](int i, float (&s)[2 * RT][PARTS]) {
-    const int k = (warp + i * WARPS) * KCHUNK;
-#pragma unroll
-    for (int r = 0; r < 2 * RT; ++r) {
-      const int n = n0 + r * 8 + g;
-#pragma unroll
-      for (int p = 0; p < PARTS; ++p) {
-        const int at = k + p * P::G;
-        s[r][p] = i < mine && n < N && at < K ? __bfloat162float(scales[(size_t)n * lds + at / P::G]) : 0.f;
-      }
+  auto next_place = [&]() {
+    at_stage = at_stage + 1 == P::STAGES ? 0 : at_stage + 1;
+    if (++at_chunk == mine) {
+      at_chunk = 0;
+      at_tile += RT;
+      if (at_tile < last) rows_of(at_tile);
     }
   };
-
-  // weights and scales depend on nothing that is computed in the step: on their way before the wait
-#pragma unroll
-  for (int s = 0; s < P::STAGES - 1; ++s)
-    if (s < mine) issue_w(s);
-  float sc[2 * RT][PARTS];
-  fetch_scales(0, sc);
-  pdl_wait();
-#pragma unroll
-  for (int s = 0; s < P::STAGES - 1; ++s) {
-    if (s < mine) issue_x(s);
-    cp_async_commit();
-  }
-  float acc[RT][NT][4];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[rt][nt][e] = 0.f;
-
-  for (int i = 0; i < mine; ++i) {
-    if (i + P::STAGES - 1 < mine) {
-      issue_w(i + P::STAGES - 1);
-      issue_x(i + P::STAGES - 1);
-    }
-    cp_async_commit();
-    float next[2 * RT][PARTS];
-    fetch_scales(i + 1, next);
-    cp_async_wait<P::STAGES - 1>();  // this thread's copies of chunk i have landed; only it reads them
-    const uint4* slot = ring + (size_t)(i % P::STAGES) * P::PIECES * THREADS + tid;
-    uint4 b[NT][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) b[nt][j] = slot[(2 * RT + nt * 4 + j) * THREADS];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const uint4 lo = slot[(2 * rt) * THREADS], hi = slot[(2 * rt + 1) * THREADS];
-      const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-      for (int p = 0; p < PARTS; ++p) {
-        float part[NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) part[nt][e] = 0.f;
-#pragma unroll
-        for (int j = p * 4 / PARTS; j < (p + 1) * 4 / PARTS; ++j) {
-          const uint32_t a[4] = {weights_of(wl[j], 0), weights_of(wl[j], 1), weights_of(wl[j], 2), weights_of(wl[j], 3)};
-          const uint32_t c[4] = {weights_of(wh[j], 0), weights_of(wh[j], 1), weights_of(wh[j], 2), weights_of(wh[j], 3)};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma(part[nt], a[0], c[0], a[1], c[1], b[nt][j].x, b[nt][j].y);
-            mma(part[nt], a[2], c[2], a[3], c[3], b[nt][j].z, b[nt][j].w);
-          }
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          acc[rt][nt][0] = fmaf(part[nt][0], sc[2 * rt][p], acc[rt][nt][0]);
-          acc[rt][nt][1] = fmaf(part[nt][1], sc[2 * rt][p], acc[rt][nt][1]);
-          acc[rt][nt][2] = fmaf(part[nt][2], sc[2 * rt + 1][p], acc[rt][nt][2]);
-          acc[rt][nt][3] = fmaf(part[nt][3], sc[2 * rt + 1][p], acc[rt][nt][3]);
-        }
-      }
-    }
+  // the scales of a chunk: rows g + 8 r of the tiles, its groups
+  auto fetch_scales = [&](int tile, int i, __nv_bfloat16 (&s)[2 * RT][PARTS]) {
 #pragma unroll
     for (int r = 0; r < 2 * RT; ++r)
 #pragma unroll
-      for (int p = 0; p < PARTS; ++p) sc[r][p] = next[r][p];
+      for (int p = 0; p < PARTS; ++p) {
+        const bool ok = tile < last && (WHOLE || (warp + i * WARPS) * KCHUNK + p * P::G < K);
+        const uint32_t at = (uint32_t)min(tile * ROWS + r * 8 + g, N - 1) * lds + (warp + i * WARPS) * PARTS + p;
+        s[r][p] = ok ? scales[at] : __float2bfloat16_rn(0.f);
+      }
+  };
+
+  // codes and scales depend on nothing that is computed in the step: on their way before the wait
+  const int total = mine * ((last - first + RT - 1) / RT);
+  {
+    const int tile = at_tile;
+#pragma unroll
+    for (int s = 0; s < P::STAGES - 1; ++s)
+      if (s < mine) issue_w(tile, s, ring + s * P::PIECES * THREADS);
   }
-  cp_async_wait<0>();
-  __syncthreads();  // the sums take the ring's memory
-  typedef float Sums[RT * ROWS][NT * 8];
-  Sums* red = reinterpret_cast<Sums*>(ring_raw);
+  __nv_bfloat16 sc[2 * RT][PARTS];
+  if (mine > 0) fetch_scales(first, 0, sc);
+  pdl_wait();
+#pragma unroll
+  for (int s = 0; s < P::STAGES - 1; ++s) {
+    if (s < total) {
+      uint4* slot = ring + s * P::PIECES * THREADS;
+      if (s >= mine) issue_w(at_tile, at_chunk, slot);
+      issue_x(at_chunk, slot);
+      next_place();
+    }
+    cp_async_commit();
+  }
+
+  float acc[RT][4];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float* at = &red[warp][rt * ROWS + g][nt * 8 + 2 * t];
-      at[0] = acc[rt][nt][0];
-      at[1] = acc[rt][nt][1];
-      at += 8 * NT * 8;
-      at[0] = acc[rt][nt][2];
-      at[1] = acc[rt][nt][3];
-    }
-  __syncthreads();
-  auto total = [&](int row, int tok) {
-    float s = 0.f;
+    for (int e = 0; e < 4; ++e) acc[rt][e] = 0.f;
+  int stage = 0, done = 0;
+  for (int tile = first; tile < last; tile += RT) {
+    for (int i = 0; i < mine; ++i, ++done) {
+      if (done + P::STAGES - 1 < total) {
+        uint4* slot = ring + at_stage * P::PIECES * THREADS;
+        issue_w(at_tile, at_chunk, slot);
+        issue_x(at_chunk, slot);
+        next_place();
+      }
+      cp_async_commit();
+      __nv_bfloat16 next[2 * RT][PARTS];
+      fetch_scales(i + 1 < mine ? tile : tile + RT, i + 1 < mine ? i + 1 : 0, next);
+      cp_async_wait<P::STAGES - 1>();  // this thread's copies of the chunk have landed; only it reads them
+      const uint4* slot = ring + stage * P::PIECES * THREADS;
+      stage = stage + 1 == P::STAGES ? 0 : stage + 1;
+      uint4 b[4];
 #pragma unroll
-    for (int wi = 0; wi < WARPS; ++wi) s += red[wi][row][tok];
-    return s;
-  };
-  if (epi.gated) {
-    for (int i = tid; i < RT * 8 * NT * 8; i += THREADS) {
-      const int tok = i / (RT * 8), f = i - tok * (RT * 8), row = f / 8 * 16 + f % 8;
-      if (tok < M && n0 + row + 8 < N) {
-        // both are rounded to bfloat16 first, as a separate gate kernel would see them
-        const float gr = __bfloat162float(__float2bfloat16_rn(total(row, tok)));
-        const float ur = __bfloat162float(__float2bfloat16_rn(total(row + 8, tok)));
-        y[(size_t)tok * ldy + n0 / 2 + f] = from_f32<TO>((epi.act ? fmaxf(gr, 0.f) : gr / (1.f + expf(-gr))) * ur);
+      for (int j = 0; j < 4; ++j) b[j] = slot[(2 * RT + j) * THREADS];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        if (rt > 0 && tile + rt >= last) break;
+        const uint4 lo = slot[(2 * rt) * THREADS], hi = slot[(2 * rt + 1) * THREADS];
+        const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+          float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = p * 4 / PARTS; j < (p + 1) * 4 / PARTS; ++j) {
+            mma(part, weights_of(wl[j], 0), weights_of(wh[j], 0), weights_of(wl[j], 1), weights_of(wh[j], 1), b[j].x, b[j].y);
+            mma(part, weights_of(wl[j], 2), weights_of(wh[j], 2), weights_of(wl[j], 3), weights_of(wh[j], 3), b[j].z, b[j].w);
+          }
+          const float s_lo = __bfloat162float(sc[2 * rt][p]), s_hi = __bfloat162float(sc[2 * rt + 1][p]);
+          acc[rt][0] = fmaf(part[0], s_lo, acc[rt][0]);
+          acc[rt][1] = fmaf(part[1], s_lo, acc[rt][1]);
+          acc[rt][2] = fmaf(part[2], s_hi, acc[rt][2]);
+          acc[rt][3] = fmaf(part[3], s_hi, acc[rt][3]);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 2 * RT; ++r)
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) sc[r][p] = next[r][p];
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      float* at = &red[warp][rt * ROWS + g][2 * t];
+      *reinterpret_cast<float2*>(at) = make_float2(acc[rt][0], acc[rt][1]);
+      *reinterpret_cast<float2*>(at + 8 * TOKENS) = make_float2(acc[rt][2], acc[rt][3]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[rt][e] = 0.f;
+    }
+    __syncthreads();
+    const int n0 = tile * ROWS, n1 = min(N, min(last, tile + RT) * ROWS);  // rows
+    auto sum = [&](int row, int tok) {
+      float v = 0.f;
+#pragma unroll
+      for (int wi = 0; wi < WARPS; ++wi) v += red[wi][row][tok];
+      return v;
+    };
+    if (epi.gated) {
+      for (int i = tid; i < RT * 8 * TOKENS; i += THREADS) {
+        const int tok = i / (RT * 8), f = i - tok * (RT * 8), row = f / 8 * 16 + f % 8;
+        if (tok < M && n0 + row + 8 < n1) {
+          // both are rounded to bfloat16 first, as a separate gate kernel would see them
+          const float gr = __bfloat162float(__float2bfloat16_rn(sum(row, tok)));
+          const float ur = __bfloat162float(__float2bfloat16_rn(sum(row + 8, tok)));
+          y[(size_t)tok * ldy + n0 / 2 + f] = from_f32<TO>((epi.act ? fmaxf(gr, 0.f) : gr / (1.f + expf(-gr))) * ur);
+        }
+      }
+    } else {
+      for (int i = tid; i < RT * ROWS * TOKENS; i += THREADS) {
+        const int tok = i / (RT * ROWS), row = i - tok * (RT * ROWS);  // consecutive threads write consecutive columns of y
+        if (tok < M && n0 + row < n1) {
+          float v = sum(row, tok);
+          if (epi.bias != nullptr) v += __bfloat162float(epi.bias[n0 + row]);
+          // the product is rounded to bfloat16 before the activation, as a separate kernel would see it
+          if (epi.act != ACT_NONE) v = activate(__bfloat162float(__float2bfloat16_rn(v)), epi.act);
+          y[(size_t)tok * ldy + n0 + row] = from_f32<TO>(v);
+        }
       }
     }
-    return;
+    if (tile + RT < last) __syncthreads();  // the sums' memory is free again
   }
-  for (int i = tid; i < RT * ROWS * NT * 8; i += THREADS) {
-    const int tok = i / (RT * ROWS), row = i - tok * (RT * ROWS);  // consecutive threads write consecutive columns of y
-    if (tok < M && n0 + row < N) {
-      float v = total(row, tok);
-      if (epi.bias != nullptr) v += __bfloat162float(epi.bias[n0 + row]);
-      // the product is rounded to bfloat16 before the activation, as a separate kernel would see it
-      if (epi.act != ACT_NONE) v = activate(__bfloat162float(__float2bfloat16_rn(v)), epi.act);
-      y[(size_t)tok * ldy + n0 + row] = from_f32<TO>(v);
-    }
-  }
+  cp_async_wait<0>();
 }
 
 template <typename P, typename TO>
@@ -234,21 +247,22 @@ int launch(const void* x, int ldx, const void* w, const void* scales, void* y, i
   auto kern = gemm_w4_kernel<P, TO>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::SMEM);
   FG_CHECK_ARG(e == cudaSuccess, "fg_gemm_w4: shared memory: %s", cudaGetErrorString(e));
-  constexpr int R = P::RT * ROWS;
-  fg_launch_pdl(kern, dim3((N + R - 1) / R), dim3(THREADS), P::SMEM, stream, (const __nv_bfloat16*)x, ldx, (const uint32_t*)w, K / 8,
-                (const __nv_bfloat16*)scales, K / P::G, (TO*)y, ldy, M, N, K, epi);
+  const int tiles = (N + ROWS - 1) / ROWS, units = (tiles + P::RT - 1) / P::RT, most = P::BLOCKS * fg_sm_count();
+  fg_launch_pdl(kern, dim3(units < most ? units : most), dim3(THREADS), P::SMEM, stream, (const __nv_bfloat16*)x, ldx,
+                (const uint32_t*)w, K / 8, (const __nv_bfloat16*)scales, K / P::G, (TO*)y, ldy, M, N, K, epi);
   return 0;
 }
 
+// Rows a block takes at a time, by the tiles of 16 rows: few ones have a block each, so that every SM gets some; many share x
+// and the loop's cost four to a block.  (us, 8 tokens, RT = 1 / 2 / 4, launches of one unit a block: 4,096 x 4,096 6.1 / 7.1 / 9.6,
+// 6,144 x 4,096 9.1 / 7.8 / 10.3, 14,336 x 4,096 18.1 / 14.3 / 11.6, 28,672 x 4,096 32.5 / 22.9 / 20.8.)
 template <int G, typename TO>
 int choose(const void* x, int ldx, const void* w, const void* scales, void* y, int ldy, int M, int N, int K, const Epilogue4& epi,
            cudaStream_t stream) {
-  const bool few = (N + ROWS - 1) / ROWS <= 2 * fg_sm_count();
-  if (M <= 8)
-    return few ? launch<Plan4<1, 1, G>, TO>(x, ldx, w, scales, y, ldy, M, N, K, epi, stream)
-               : launch<Plan4<2, 1, G>, TO>(x, ldx, w, scales, y, ldy, M, N, K, epi, stream);
-  return few ? launch<Plan4<1, 2, G>, TO>(x, ldx, w, scales, y, ldy, M, N, K, epi, stream)
-             : launch<Plan4<2, 2, G>, TO>(x, ldx, w, scales, y, ldy, M, N, K, epi, stream);
+  const int tiles = (N + ROWS - 1) / ROWS;
+  if (tiles <= 2 * fg_sm_count()) return launch<Plan4<1, G>, TO>(x, ldx, w, scales, y, ldy, M, N, K, epi, stream);
+  if (tiles <= 4 * fg_sm_count()) return launch<Plan4<2, G>, TO>(x, ldx, w, scales, y, ldy, M, N, K, epi, stream);
+  return launch<Plan4<4, G>, TO>(x, ldx, w, scales, y, ldy, M, N, K, epi, stream);
 }
 
 template <typename TO>
@@ -295,7 +309,7 @@ extern "C" int fg_w4_dense(const void* w, const void* scales, int group, void* o
   return 0;
 }
 
-extern "C" int fg_gemm_w4_max_m() { return 16; }
+extern "C" int fg_gemm_w4_max_m() { return TOKENS; }
 
 // x: [M, K] bf16 (row stride ldx); w: codes [N, K / 8] words (see above); scales: bf16 [N, K / group]; y: [M, N] bf16 or float32,
 // or with `gated` [M, N / 2] bf16: silu (relu with act 1) of the gate rows times the up rows, which lie in blocks of 8 in
@@ -303,10 +317,11 @@ extern "C" int fg_gemm_w4_max_m() { return 16; }
 extern "C" int fg_gemm_w4(const void* x, int ldx, const void* w, const void* scales, int group, void* y, int ldy, int out_dtype,
                           int M, int N, int K, const void* bias, int act, int gated, cudaStream_t stream) {
   if (M == 0 || N == 0) return 0;
-  FG_CHECK_ARG(M <= 16, "fg_gemm_w4: M=%d exceeds 16", M);
+  FG_CHECK_ARG(M <= TOKENS, "fg_gemm_w4: M=%d exceeds %d", M, TOKENS);
   FG_CHECK_ARG(group == 32 || group == 64 || group == 128, "fg_gemm_w4: groups of %d columns are not supported (32, 64, 128)", group);
   FG_CHECK_ARG(K > 0 && K % group == 0, "fg_gemm_w4: K=%d is no multiple of the group of %d", K, group);
   FG_CHECK_ARG(ldx % 8 == 0 && ldx >= K && ldy >= (gated ? N / 2 : N), "fg_gemm_w4: row strides %d and %d", ldx, ldy);
+  FG_CHECK_ARG((long long)N * (K / 8) < (1ll << 32) && (long long)M * ldx < (1ll << 32), "fg_gemm_w4: N=%d K=%d too large", N, K);
   FG_CHECK_ARG((((uintptr_t)x | (uintptr_t)w) & 15) == 0, "fg_gemm_w4: x and the codes must be 16-byte aligned");
   FG_CHECK_ARG(!gated || (N % 16 == 0 && bias == nullptr && out_dtype == FG_BF16), "fg_gemm_w4: a gated product of %d rows", N);
   FG_CHECK_ARG(act >= ACT_NONE && act <= ACT_RELU2, "fg_gemm_w4: unknown activation %d", act);

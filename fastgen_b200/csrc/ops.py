@@ -134,7 +134,7 @@ _ATTN_SIGNATURES = {
 }
 
 SKINNY_MAX_M = int(os.environ.get("FG_SKINNY_MAX_M", "8"))      # most tokens the weight-streaming product is used for (it takes up to 32)
-W4_MAX_M = 16        # tokens a launch of the product that streams 4-bit weights takes
+W4_MAX_M = 8         # most tokens of the product that streams 4-bit weights; more go to tcgen05
 W4_DENSE_M = 256     # tokens from which 4-bit weights are expanded for the product of 16-bit ones
 SIMT_ROWS = 16       # query rows per block of the float32 attention kernel
 F32_PROMPT_ROWS = 64  # ... of the float32 kernel of larger prompts
@@ -1463,7 +1463,7 @@ class Ops(Kv8Ops):
 
         A ``memory`` with scales is a cache in 8 bits (bfloat16 only): single tokens in a kernel of their own, for prompt
         portions the pages they read are expanded to bfloat16 (exactly) and the kernels above run on those."""
-        if memory.k_scales is not None:
+        if getattr(memory, "k_scales", None) is not None:
             return self._attention_kv8(q, out, memory, ctx, n_heads, n_kv_heads, head_dim, window, scale, out_freqs,
                                        keep_first, softcap, sinks, chunk)
         lib = attn(head_dim)

@@ -242,7 +242,8 @@ class GQAAttention(Mixer):
         t = x.shape[0]
         q = None
         gate = None
-        if memory.writes and x.dtype == torch.bfloat16 and self.plain and memory.k_scales is None and not isinstance(self.wqkv, Weight4):
+        in_8_bits = getattr(memory, "k_scales", None) is not None
+        if memory.writes and x.dtype == torch.bfloat16 and self.plain and not in_8_bits and not isinstance(self.wqkv, Weight4):
             # a few tokens: projection, rotation and page write in one kernel
             q = ops.qkv_rope_write(x, self.wqkv, ctx.pos, ctx.req, self.freqs, memory,
                                    p.n_heads, p.n_kv_heads, self.hd, bias=self.bqkv, v_freqs=self.v_freqs)
@@ -278,7 +279,7 @@ class GQAAttention(Mixer):
                 # that rotates multiplies by them and by the weights
                 rstd = ops.qk_rstd(q, k, p.n_heads * p.head_dim, p.n_kv_heads * p.head_dim, p.qk_norm_eps, ctx.req)
                 qk_norm = (rstd, self.q_norm, self.k_norm)
-            if memory.writes and memory.k_scales is not None:
+            if memory.writes and in_8_bits:
                 q = ops.rope_kv8_write(q, k, v, ctx.pos, ctx.req, self.freqs, memory, p.n_heads, p.n_kv_heads, self.hd,
                                        v_freqs=self.v_freqs, qk_norm=qk_norm, magnitude=self.magnitude, rot_pairs=self.rot_pairs)
             else:
