@@ -4,13 +4,15 @@
 //
 // Bound by reading the codes once, half a byte a weight.  As in gemm_skinny.cu, 16 rows of W are the "M" side of
 // mma.sync m16n8k16 and 8 tokens its "N" side, a thread streams its own pieces through a ring of cp.async stages that only it
-// reads back, and the block's eight warps split K in chunks of 128 that are summed in warp order at the end.
+// reads back, and the eight warps of a block, or of each block of a cluster, split K in chunks of 128 that are summed in a fixed order.
 //  * A 32-bit word holds eight columns of a row, the even columns in its low half's nibbles and the odd ones in its
 //    high half's: the nibbles at bit 4 i of both halves are columns 2 i and 2 i + 1, so that one `and-or` with 0x4300 (128 in
 //    bfloat16, whose last bit is then 1) makes the pair 128 + code of an operand register and one subtraction code - 8: 11
 //    instructions for eight weights, all of them exact.
 //  * The weights enter the product as the whole numbers they are; a group's sums are multiplied by the group's scale in
 //    float32 on their way into the accumulators.  Nothing is rounded to 16 bits but the result.
+//  * What it spends (28,672 x 4,096, one token, 19 us): the copies alone take 11.4, the products and scales add the rest; two
+//    blocks an SM do not hide all of one another's waits.
 //  * In a chunk a lane takes 32 neighbouring columns (one 16-byte piece a row).  Groups of 32 and 64 columns must not meet in
 //    one instruction: there the four lanes of a row take a word each of the same 32 columns, four pieces of four bytes.
 #include "skinny_product.cuh"
@@ -21,6 +23,7 @@ using namespace fg_skinny;
 
 constexpr int KCHUNK = 128;  // columns a warp takes at a time
 constexpr int TOKENS = 8;
+constexpr int MAX_SHARE = 4;  // blocks of a cluster that split K
 
 __device__ __forceinline__ void cp_async_4(void* dst, const void* src, bool pred) {
   const int bytes = pred ? 4 : 0;
@@ -36,7 +39,7 @@ __device__ __forceinline__ uint32_t weights_of(uint32_t w, int i) {
   return *reinterpret_cast<const uint32_t*>(&d);
 }
 
-// RT tiles of 16 rows at a time a block; G columns a group
+// RT tiles of 16 rows a block; G columns a group
 template <int RT_, int G_>
 struct Plan4 {
   static constexpr int RT = RT_, G = G_;
@@ -48,55 +51,57 @@ struct Plan4 {
   static constexpr int BLOCKS = SMEM <= 75 * 1024 ? 3 : 2;  // an SM
 };
 
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
+  uint32_t remote;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(remote) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(remote) : "memory");
+  return v;
+}
+
 struct Epilogue4 {
   const __nv_bfloat16* bias;  // [N] or null
   int act;                    // ACT_*; with `gated`: 1 for a relu gate
   bool gated;                 // rows are gate and up in blocks of 8: y[M, N / 2]
 };
 
-// A block works on a stretch of neighbouring tiles of 16 rows, an equal share of all, RT at a time; the copies of the next
-// ones run while the sums of the last are stored.
 template <typename P, typename TO>
 __global__ void __launch_bounds__(THREADS, P::BLOCKS)
 gemm_w4_kernel(const __nv_bfloat16* x, int ldx, const uint32_t* __restrict__ w, int ldw, const __nv_bfloat16* __restrict__ scales,
-               int lds, TO* __restrict__ y, int ldy, int M, int N, int K, Epilogue4 epi) {
+               int lds, TO* __restrict__ y, int ldy, int M, int N, int K, int share, Epilogue4 epi) {
   constexpr int RT = P::RT, PARTS = KCHUNK / P::G;  // groups of a chunk
   // Rows beyond N and tokens beyond M are read as the last ones and left out of the result; K is whole chunks where the
   // groups are (WHOLE), else columns beyond K are zeros.
   constexpr bool WHOLE = P::G == KCHUNK;
-  constexpr int STEP = WARPS * KCHUNK;  // columns from one of the warp's chunks to its next
   extern __shared__ __align__(16) unsigned char ring_raw[];
   uint4* const ring = reinterpret_cast<uint4*>(ring_raw) + threadIdx.x;  // [STAGES][PIECES][THREADS]
   typedef float Sums[RT * ROWS][TOKENS];
   Sums* const red = reinterpret_cast<Sums*>(ring_raw + P::RING);  // [WARPS]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int tiles = (N + ROWS - 1) / ROWS;
-  const int first = (int)((long long)tiles * blockIdx.x / gridDim.x), last = (int)((long long)tiles * (blockIdx.x + 1) / gridDim.x);
-  const int n_chunks = (K + KCHUNK - 1) / KCHUNK;
-  const int mine = warp < n_chunks ? (n_chunks - warp + WARPS - 1) / WARPS : 0;  // of this warp, of every tile
+  const int rank = blockIdx.x % share, n0 = blockIdx.x / share * RT * ROWS;
+  // chunk c is the cluster's warp c mod (8 share)'s: `mine` of them from `first` on, `step` apart
+  const int n_chunks = (K + KCHUNK - 1) / KCHUNK, first = rank * WARPS + warp, step = share * WARPS;
+  const int mine = first < n_chunks ? (n_chunks - first + step - 1) / step : 0;
   pdl_trigger();
 
-  // the copies' place: tile, this warp's chunk of it, stage
-  int at_tile = first, at_chunk = 0, at_stage = 0;
   uint32_t w_row[2 * RT];
-  auto rows_of = [&](int tile) {
 #pragma unroll
-    for (int r = 0; r < 2 * RT; ++r)
-      w_row[r] = (uint32_t)min(tile * ROWS + r * 8 + g, N - 1) * ldw + warp * (KCHUNK / 8) + (WHOLE ? 4 * t : t);
-  };
-  rows_of(first);
-  const uint32_t x_row = (uint32_t)min(g, M - 1) * ldx + warp * KCHUNK + (WHOLE ? 32 * t : 8 * t);
-  auto issue_w = [&](int tile, int i, uint4* slot) {
+  for (int r = 0; r < 2 * RT; ++r)
+    w_row[r] = (uint32_t)min(n0 + r * 8 + g, N - 1) * ldw + first * (KCHUNK / 8) + (WHOLE ? 4 * t : t);
+  const uint32_t x_row = (uint32_t)min(g, M - 1) * ldx + first * KCHUNK + (WHOLE ? 32 * t : 8 * t);
+  auto issue_w = [&](int i, uint4* slot) {
 #pragma unroll
     for (int r = 0; r < 2 * RT; ++r) {
-      if (r >= 2 && tile + r / 2 >= last) break;  // (the stretch's last tiles may be fewer than RT)
       if (WHOLE) {
-        cp_async_16<false>(slot + r * THREADS, w + (w_row[r] + i * (STEP / 8)), true);
+        cp_async_16<false>(slot + r * THREADS, w + (w_row[r] + i * (step * (KCHUNK / 8))), true);
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const bool ok = (warp + i * WARPS) * KCHUNK + 32 * j + 8 * t < K;
-          cp_async_4(reinterpret_cast<uint32_t*>(slot + r * THREADS) + j, w + (ok ? w_row[r] + i * (STEP / 8) + 4 * j : 0u), ok);
+          const bool ok = (first + i * step) * KCHUNK + 32 * j + 8 * t < K;
+          cp_async_4(reinterpret_cast<uint32_t*>(slot + r * THREADS) + j, w + (ok ? w_row[r] + i * (step * (KCHUNK / 8)) + 4 * j : 0u), ok);
         }
       }
     }
@@ -104,49 +109,32 @@ gemm_w4_kernel(const __nv_bfloat16* x, int ldx, const uint32_t* __restrict__ w, 
   auto issue_x = [&](int i, uint4* slot) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const bool ok = WHOLE || (warp + i * WARPS) * KCHUNK + 32 * j + 8 * t < K;
-      cp_async_16<true>(slot + (2 * RT + j) * THREADS, x + (ok ? x_row + i * STEP + (WHOLE ? 8 * j : 32 * j) : 0u), ok);
-    }
-  };
-  auto next_place = [&]() {
-    at_stage = at_stage + 1 == P::STAGES ? 0 : at_stage + 1;
-    if (++at_chunk == mine) {
-      at_chunk = 0;
-      at_tile += RT;
-      if (at_tile < last) rows_of(at_tile);
+      const bool ok = WHOLE || (first + i * step) * KCHUNK + 32 * j + 8 * t < K;
+      cp_async_16<true>(slot + (2 * RT + j) * THREADS, x + (ok ? x_row + i * (step * KCHUNK) + (WHOLE ? 8 * j : 32 * j) : 0u), ok);
     }
   };
   // the scales of a chunk: rows g + 8 r of the tiles, its groups
-  auto fetch_scales = [&](int tile, int i, __nv_bfloat16 (&s)[2 * RT][PARTS]) {
+  auto fetch_scales = [&](int i, __nv_bfloat16 (&s)[2 * RT][PARTS]) {
 #pragma unroll
     for (int r = 0; r < 2 * RT; ++r)
 #pragma unroll
       for (int p = 0; p < PARTS; ++p) {
-        const bool ok = tile < last && (WHOLE || (warp + i * WARPS) * KCHUNK + p * P::G < K);
-        const uint32_t at = (uint32_t)min(tile * ROWS + r * 8 + g, N - 1) * lds + (warp + i * WARPS) * PARTS + p;
+        const bool ok = i < mine && (WHOLE || (first + i * step) * KCHUNK + p * P::G < K);
+        const uint32_t at = (uint32_t)min(n0 + r * 8 + g, N - 1) * lds + (first + i * step) * PARTS + p;
         s[r][p] = ok ? scales[at] : __float2bfloat16_rn(0.f);
       }
   };
 
   // codes and scales depend on nothing that is computed in the step: on their way before the wait
-  const int total = mine * ((last - first + RT - 1) / RT);
-  {
-    const int tile = at_tile;
 #pragma unroll
-    for (int s = 0; s < P::STAGES - 1; ++s)
-      if (s < mine) issue_w(tile, s, ring + s * P::PIECES * THREADS);
-  }
+  for (int s = 0; s < P::STAGES - 1; ++s)
+    if (s < mine) issue_w(s, ring + s * P::PIECES * THREADS);
   __nv_bfloat16 sc[2 * RT][PARTS];
-  if (mine > 0) fetch_scales(first, 0, sc);
+  fetch_scales(0, sc);
   pdl_wait();
 #pragma unroll
   for (int s = 0; s < P::STAGES - 1; ++s) {
-    if (s < total) {
-      uint4* slot = ring + s * P::PIECES * THREADS;
-      if (s >= mine) issue_w(at_tile, at_chunk, slot);
-      issue_x(at_chunk, slot);
-      next_place();
-    }
+    if (s < mine) issue_x(s, ring + s * P::PIECES * THREADS);
     cp_async_commit();
   }
 
@@ -155,114 +143,150 @@ gemm_w4_kernel(const __nv_bfloat16* x, int ldx, const uint32_t* __restrict__ w, 
   for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[rt][e] = 0.f;
-  int stage = 0, done = 0;
-  for (int tile = first; tile < last; tile += RT) {
-    for (int i = 0; i < mine; ++i, ++done) {
-      if (done + P::STAGES - 1 < total) {
-        uint4* slot = ring + at_stage * P::PIECES * THREADS;
-        issue_w(at_tile, at_chunk, slot);
-        issue_x(at_chunk, slot);
-        next_place();
-      }
-      cp_async_commit();
-      __nv_bfloat16 next[2 * RT][PARTS];
-      fetch_scales(i + 1 < mine ? tile : tile + RT, i + 1 < mine ? i + 1 : 0, next);
-      cp_async_wait<P::STAGES - 1>();  // this thread's copies of the chunk have landed; only it reads them
-      const uint4* slot = ring + stage * P::PIECES * THREADS;
-      stage = stage + 1 == P::STAGES ? 0 : stage + 1;
-      uint4 b[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) b[j] = slot[(2 * RT + j) * THREADS];
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        if (rt > 0 && tile + rt >= last) break;
-        const uint4 lo = slot[(2 * rt) * THREADS], hi = slot[(2 * rt + 1) * THREADS];
-        const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) {
-          float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int j = p * 4 / PARTS; j < (p + 1) * 4 / PARTS; ++j) {
-            mma(part, weights_of(wl[j], 0), weights_of(wh[j], 0), weights_of(wl[j], 1), weights_of(wh[j], 1), b[j].x, b[j].y);
-            mma(part, weights_of(wl[j], 2), weights_of(wh[j], 2), weights_of(wl[j], 3), weights_of(wh[j], 3), b[j].z, b[j].w);
-          }
-          const float s_lo = __bfloat162float(sc[2 * rt][p]), s_hi = __bfloat162float(sc[2 * rt + 1][p]);
-          acc[rt][0] = fmaf(part[0], s_lo, acc[rt][0]);
-          acc[rt][1] = fmaf(part[1], s_lo, acc[rt][1]);
-          acc[rt][2] = fmaf(part[2], s_hi, acc[rt][2]);
-          acc[rt][3] = fmaf(part[3], s_hi, acc[rt][3]);
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < 2 * RT; ++r)
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) sc[r][p] = next[r][p];
+  int stage = 0, free = P::STAGES - 1;
+  for (int i = 0; i < mine; ++i) {
+    if (i + P::STAGES - 1 < mine) {
+      issue_w(i + P::STAGES - 1, ring + free * P::PIECES * THREADS);
+      issue_x(i + P::STAGES - 1, ring + free * P::PIECES * THREADS);
     }
+    cp_async_commit();
+    free = free + 1 == P::STAGES ? 0 : free + 1;
+    __nv_bfloat16 next[2 * RT][PARTS];
+    fetch_scales(i + 1, next);
+    cp_async_wait<P::STAGES - 1>();  // this thread's copies of the chunk have landed; only it reads them
+    const uint4* slot = ring + stage * P::PIECES * THREADS;
+    stage = stage + 1 == P::STAGES ? 0 : stage + 1;
+    uint4 b[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) b[j] = slot[(2 * RT + j) * THREADS];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      float* at = &red[warp][rt * ROWS + g][2 * t];
-      *reinterpret_cast<float2*>(at) = make_float2(acc[rt][0], acc[rt][1]);
-      *reinterpret_cast<float2*>(at + 8 * TOKENS) = make_float2(acc[rt][2], acc[rt][3]);
+      const uint4 lo = slot[(2 * rt) * THREADS], hi = slot[(2 * rt + 1) * THREADS];
+      const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[rt][e] = 0.f;
+      for (int p = 0; p < PARTS; ++p) {
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = p * 4 / PARTS; j < (p + 1) * 4 / PARTS; ++j) {
+          mma(part, weights_of(wl[j], 0), weights_of(wh[j], 0), weights_of(wl[j], 1), weights_of(wh[j], 1), b[j].x, b[j].y);
+          mma(part, weights_of(wl[j], 2), weights_of(wh[j], 2), weights_of(wl[j], 3), weights_of(wh[j], 3), b[j].z, b[j].w);
+        }
+        const float s_lo = __bfloat162float(sc[2 * rt][p]), s_hi = __bfloat162float(sc[2 * rt + 1][p]);
+        acc[rt][0] = fmaf(part[0], s_lo, acc[rt][0]);
+        acc[rt][1] = fmaf(part[1], s_lo, acc[rt][1]);
+        acc[rt][2] = fmaf(part[2], s_hi, acc[rt][2]);
+        acc[rt][3] = fmaf(part[3], s_hi, acc[rt][3]);
+      }
     }
-    __syncthreads();
-    const int n0 = tile * ROWS, n1 = min(N, min(last, tile + RT) * ROWS);  // rows
-    auto sum = [&](int row, int tok) {
+#pragma unroll
+    for (int r = 0; r < 2 * RT; ++r)
+#pragma unroll
+      for (int p = 0; p < PARTS; ++p) sc[r][p] = next[r][p];
+  }
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    float* at = &red[warp][rt * ROWS + g][2 * t];
+    *reinterpret_cast<float2*>(at) = make_float2(acc[rt][0], acc[rt][1]);
+    *reinterpret_cast<float2*>(at + 8 * TOKENS) = make_float2(acc[rt][2], acc[rt][3]);
+  }
+  __syncthreads();
+  // the block's warps in turn; then, over distributed shared memory, the cluster's blocks
+  float* const part = reinterpret_cast<float*>(ring_raw);  // [RT * ROWS * TOKENS]: every warp has read its copies by now
+  if (share > 1) {
+    for (int i = tid; i < RT * ROWS * TOKENS; i += THREADS) {
       float v = 0.f;
 #pragma unroll
+      for (int wi = 0; wi < WARPS; ++wi) v += (&red[wi][0][0])[i];
+      part[i] = v;
+    }
+    cluster_sync();
+  }
+  auto sum = [&](int row, int tok) {
+    float v = 0.f;
+    if (share == 1) {
+#pragma unroll
       for (int wi = 0; wi < WARPS; ++wi) v += red[wi][row][tok];
-      return v;
-    };
-    if (epi.gated) {
-      for (int i = tid; i < RT * 8 * TOKENS; i += THREADS) {
-        const int tok = i / (RT * 8), f = i - tok * (RT * 8), row = f / 8 * 16 + f % 8;
-        if (tok < M && n0 + row + 8 < n1) {
-          // both are rounded to bfloat16 first, as a separate gate kernel would see them
-          const float gr = __bfloat162float(__float2bfloat16_rn(sum(row, tok)));
-          const float ur = __bfloat162float(__float2bfloat16_rn(sum(row + 8, tok)));
-          y[(size_t)tok * ldy + n0 / 2 + f] = from_f32<TO>((epi.act ? fmaxf(gr, 0.f) : gr / (1.f + expf(-gr))) * ur);
-        }
-      }
     } else {
-      for (int i = tid; i < RT * ROWS * TOKENS; i += THREADS) {
-        const int tok = i / (RT * ROWS), row = i - tok * (RT * ROWS);  // consecutive threads write consecutive columns of y
-        if (tok < M && n0 + row < n1) {
-          float v = sum(row, tok);
-          if (epi.bias != nullptr) v += __bfloat162float(epi.bias[n0 + row]);
-          // the product is rounded to bfloat16 before the activation, as a separate kernel would see it
-          if (epi.act != ACT_NONE) v = activate(__bfloat162float(__float2bfloat16_rn(v)), epi.act);
-          y[(size_t)tok * ldy + n0 + row] = from_f32<TO>(v);
-        }
+      const uint32_t at = smem_u32(part + row * TOKENS + tok);
+      float p[MAX_SHARE];
+#pragma unroll
+      for (int b = 0; b < MAX_SHARE; ++b) p[b] = b < share ? ld_cluster(at, b) : 0.f;
+#pragma unroll
+      for (int b = 0; b < MAX_SHARE; ++b) v += p[b];
+    }
+    return v;
+  };
+  if (epi.gated) {
+    for (int i = rank * THREADS + tid; i < RT * 8 * TOKENS; i += share * THREADS) {
+      const int tok = i / (RT * 8), f = i - tok * (RT * 8), row = f / 8 * 16 + f % 8;
+      if (tok < M && n0 + row + 8 < N) {
+        // both are rounded to bfloat16 first, as a separate gate kernel would see them
+        const float gr = __bfloat162float(__float2bfloat16_rn(sum(row, tok)));
+        const float ur = __bfloat162float(__float2bfloat16_rn(sum(row + 8, tok)));
+        y[(size_t)tok * ldy + n0 / 2 + f] = from_f32<TO>((epi.act ? fmaxf(gr, 0.f) : gr / (1.f + expf(-gr))) * ur);
       }
     }
-    if (tile + RT < last) __syncthreads();  // the sums' memory is free again
+  } else {
+    for (int i = rank * THREADS + tid; i < RT * ROWS * TOKENS; i += share * THREADS) {
+      const int tok = i / (RT * ROWS), row = i - tok * (RT * ROWS);  // consecutive threads write consecutive columns of y
+      if (tok < M && n0 + row < N) {
+        float v = sum(row, tok);
+        if (epi.bias != nullptr) v += __bfloat162float(epi.bias[n0 + row]);
+        // the product is rounded to bfloat16 before the activation, as a separate kernel would see it
+        if (epi.act != ACT_NONE) v = activate(__bfloat162float(__float2bfloat16_rn(v)), epi.act);
+        y[(size_t)tok * ldy + n0 + row] = from_f32<TO>(v);
+      }
+    }
   }
-  cp_async_wait<0>();
+  if (share > 1) cluster_sync();  // nobody leaves while its sums are being read
 }
 
 template <typename P, typename TO>
-int launch(const void* x, int ldx, const void* w, const void* scales, void* y, int ldy, int M, int N, int K, const Epilogue4& epi,
-           cudaStream_t stream) {
+int launch(const void* x, int ldx, const void* w, const void* scales, void* y, int ldy, int M, int N, int K, int share,
+           const Epilogue4& epi, cudaStream_t stream) {
   auto kern = gemm_w4_kernel<P, TO>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::SMEM);
   FG_CHECK_ARG(e == cudaSuccess, "fg_gemm_w4: shared memory: %s", cudaGetErrorString(e));
-  const int tiles = (N + ROWS - 1) / ROWS, units = (tiles + P::RT - 1) / P::RT, most = P::BLOCKS * fg_sm_count();
-  fg_launch_pdl(kern, dim3(units < most ? units : most), dim3(THREADS), P::SMEM, stream, (const __nv_bfloat16*)x, ldx,
-                (const uint32_t*)w, K / 8, (const __nv_bfloat16*)scales, K / P::G, (TO*)y, ldy, M, N, K, epi);
+  const int units = (N + P::RT * ROWS - 1) / (P::RT * ROWS);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(units * share));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = P::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = fg_pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = share;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = share > 1 ? 2 : 1;
+  const cudaError_t le = cudaLaunchKernelEx(&cfg, kern, (const __nv_bfloat16*)x, ldx, (const uint32_t*)w, K / 8,
+                                            (const __nv_bfloat16*)scales, K / P::G, (TO*)y, ldy, M, N, K, share, epi);
+  FG_CHECK_ARG(le == cudaSuccess, "fg_gemm_w4: launch failed: %s", cudaGetErrorString(le));
   return 0;
 }
 
-// Rows a block takes at a time, by the tiles of 16 rows: few ones have a block each, so that every SM gets some; many share x
-// and the loop's cost four to a block.  (us, 8 tokens, RT = 1 / 2 / 4, launches of one unit a block: 4,096 x 4,096 6.1 / 7.1 / 9.6,
-// 6,144 x 4,096 9.1 / 7.8 / 10.3, 14,336 x 4,096 18.1 / 14.3 / 11.6, 28,672 x 4,096 32.5 / 22.9 / 20.8.)
+// Blocks cost more than rows do: a call wants between one and two of them an SM, all resident at once, each with as many rows
+// as that leaves, since the rows of a block share its copies of x.  Long rows are split over the blocks of a cluster, as long
+// as each warp keeps two chunks.  us for 8 tokens, by row tiles a block / blocks a cluster (192 to 256 blocks in the first
+// two of a line):
+//   4,096 x 4,096: 2/2 5.8, 1/1 6.4, 4/1 9.9;  4,096 x 14,336: 4/4 14.0, 1/1 18.3, 4/1 28.7;  8,192 x 8,192: 4/2 13.1, 2/1 15.6,
+//   4/1 20.7;  6,144 x 4,096: 4/2 8.6, 2/1 8.6, 1/1 10.0, 4/4 11.9;  14,336 x 4,096: 4/1 12.6, 2/1 16.5, 1/1 20.9.
 template <int G, typename TO>
 int choose(const void* x, int ldx, const void* w, const void* scales, void* y, int ldy, int M, int N, int K, const Epilogue4& epi,
            cudaStream_t stream) {
-  const int tiles = (N + ROWS - 1) / ROWS;
-  if (tiles <= 2 * fg_sm_count()) return launch<Plan4<1, G>, TO>(x, ldx, w, scales, y, ldy, M, N, K, epi, stream);
-  if (tiles <= 4 * fg_sm_count()) return launch<Plan4<2, G>, TO>(x, ldx, w, scales, y, ldy, M, N, K, epi, stream);
-  return launch<Plan4<4, G>, TO>(x, ldx, w, scales, y, ldy, M, N, K, epi, stream);
+  const int tiles = (N + ROWS - 1) / ROWS, chunks = (K + KCHUNK - 1) / KCHUNK, sms = fg_sm_count();
+  int rt = 4, share;
+  for (;; rt /= 2) {
+    const int units = (tiles + rt - 1) / rt;
+    share = 1;
+    while (share < MAX_SHARE && units * share * 2 <= 2 * sms && chunks >= 2 * WARPS * share * 2) share *= 2;
+    if (rt == 1 || units * share >= sms) break;
+  }
+  if (rt == 4) return launch<Plan4<4, G>, TO>(x, ldx, w, scales, y, ldy, M, N, K, share, epi, stream);
+  if (rt == 2) return launch<Plan4<2, G>, TO>(x, ldx, w, scales, y, ldy, M, N, K, share, epi, stream);
+  return launch<Plan4<1, G>, TO>(x, ldx, w, scales, y, ldy, M, N, K, share, epi, stream);
 }
 
 template <typename TO>
@@ -274,7 +298,7 @@ int by_group(int group, const void* x, int ldx, const void* w, const void* scale
 }
 
 // The matrix in bfloat16, for products of many tokens: a thread eight columns.  Bound by its bytes: half of one read and two
-// written a weight (28,672 x 4,096: FIGURE_X).
+// written a weight.
 __global__ void __launch_bounds__(256)
 dense_kernel(const uint32_t* __restrict__ w, const __nv_bfloat16* __restrict__ scales, int group_words, uint4* out, size_t words) {
   pdl_trigger();

@@ -13,8 +13,8 @@
 // Where the tiles are too few for the chip a cluster of 2, 4 or 8 blocks shares one: each sums a stretch of K, and they add up
 // over distributed shared memory in the order of the stretches.
 //
-// What bounds it: few tokens: reading the codes; the workers' instructions (11 for eight weights) come to about two thirds of
-// what the SM issues meanwhile.
+// What bounds it: the workers, who unpack the codes (11 instructions for eight weights) and scale the sums in turn: 28,672 x
+// 4,096 takes 25 us with 16 tokens, 30 with 64 (reading the codes 9.3, the products with 64 tokens 9.0), 57 with 128.
 #include <type_traits>
 
 #include "skinny_product.cuh"
@@ -416,13 +416,17 @@ int launch(const void* x, int ldx, const void* w, const void* scales, void* y, i
   return 0;
 }
 
-// How many blocks share a tile: as many as the chip has room for, each with two stages of codes or more.
+// How many blocks share a tile: as many as give every SM one, each with a stage of codes or more; a second block an SM only
+// where they keep four stages each.  (us by blocks a tile, 16 tokens: 4,096 x 4,096 2 / 4 / 8: 10.6 / 6.8 / 8.1; 4,096 x 14,336
+// 28.3 / 16.0 / 15.4; 6,144 x 4,096 10.7 / 9.8 / 11.3; 28,672 x 4,096 1 / 2: 25.3 / 30.7.)
 template <typename S>
 int share_of(int M, int N, int K) {
   const long tiles = (long)((M + S::T - 1) / S::T) * ((N + ROWS4 - 1) / ROWS4);
-  const int stages = (K + W_COLS - 1) / W_COLS;
+  const int stages = (K + W_COLS - 1) / W_COLS, sms = fg_sm_count();
   int share = 1;
-  while (share < 8 && tiles * share * 2 <= (long)S::BLOCKS * fg_sm_count() && stages >= 4 * share) share *= 2;
+  while (share < 8 && ((tiles * share * 2 <= sms && stages >= share * 2) ||
+                       (tiles * share * 2 <= (long)S::BLOCKS * sms && stages >= share * 8)))
+    share *= 2;
   return share;
 }
 
