@@ -79,7 +79,7 @@ extern "C" int fg_kv8_values(const void* k_pages, const void* v_pages, const flo
 extern "C" int fg_kv8_expand(const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
                              const int* block_table, int table_width, const int* seq_slot, const int* seq_start,
                              const int* seq_cached, int n_seqs, void* k_out, void* v_out, int page_size, int n_pages,
-                             int n_kv_heads, int head_dim, int window, int keep_first, int* status, cudaStream_t stream) {
+                             int n_kv_heads, int head_dim, int window, int* status, cudaStream_t stream) {
   using namespace fg_kv8;
   if (n_seqs == 0) return 0;
   if (check_pages("fg_kv8_expand", k_pages, v_pages, k_scales, v_scales, page_size, n_pages, n_kv_heads, head_dim)) return -1;
@@ -87,7 +87,7 @@ extern "C" int fg_kv8_expand(const void* k_pages, const void* v_pages, const flo
   fg_launch_pdl(kv8_expand_kernel<FG_HEAD_DIM>, dim3(8 * fg_sm_count()), dim3(EXPAND_THREADS), 0, stream,
                 (const unsigned char*)k_pages, (const unsigned char*)v_pages, k_scales, v_scales, block_table, table_width,
                 seq_slot, seq_start, seq_cached, n_seqs, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, page_size, n_pages,
-                n_kv_heads, window, window > 0 ? keep_first : 0, status);
+                n_kv_heads, window, status);
   FG_CHECK_LAUNCH("fg_kv8_expand");
   return 0;
 }

@@ -6,7 +6,7 @@
 // result; the others leave a partial (two a block at most), and the block whose partial of a request and head is counted last
 // merges them in the order of the keys: one launch, nobody waits, the order of the sums is the walk's.  (A partial for
 // every 128 keys and a merge in a launch of its own: 64 ragged requests of up to 2,800 keys, 32 / 8 heads of 128, 62.6 us
-// against 44.2, batch 8 at 4,096 keys 21.1 against 17.5.)
+// against 45.7, batch 8 at 4,096 keys 21.1 against 17.7.)
 // A producer warp streams codes through a ring of shared-memory slots ahead of four consumer warps.  In the first product a
 // consumer warp has 32 keys; the weights go to shared memory, and in the second product it has a quarter of the dimensions
 // of all 128 keys, so that there are no sums of warps to merge.
@@ -254,9 +254,6 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
 
   if (warp == 4) {
     // ================================ producer ================================
-    // The step's own kernels write the page that holds the token's position (its cached entries may be rounded again at a
-    // larger scale): splits that end before that page are loaded without waiting for them.
-    bool waited = false;
     auto page_of = [&](const Walk& w) {  // lane i: the page of box i of the item's split, or -1
       int page = -1;
       const int j0 = (w.first + w.split) * SPLIT + lane * box_rows;
@@ -272,13 +269,13 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     };
     Walk w = start();
     int page = count > 0 ? page_of(w) : -1;
+    // Any page may be what a kernel ahead has just written: nothing is loaded before those are over.  (Loading the splits
+    // before the token's own page earlier saved 0.4 us of 7.4 for a short request, 1.9 of 50.6 for 64 ragged ones, and read
+    // stale pages where a prompt's write is followed at once.)
+    pdl_wait();
     int slot = 0, use = 0;
     for (int i = 0; i < count; ++i) {
       const int k0 = (w.first + w.split) * SPLIT, g = w.slice / n_sub;
-      if (!waited && k0 + SPLIT > (w.p >> page_shift << page_shift)) {
-        pdl_wait();
-        waited = true;
-      }
       const size_t block = (size_t)max(page, 0) * n_kv_heads + g;
       const uint32_t ks = page >= 0 ? ld_global_4(k_scales + block) : 0u, vs = page >= 0 ? ld_global_4(v_scales + block) : 0u;
       // the next item's pages are on their way meanwhile
@@ -310,7 +307,6 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
       }
       page = next_page;
     }
-    if (!waited) pdl_wait();
   } else {
     // ================================ consumers ================================
     pdl_wait();

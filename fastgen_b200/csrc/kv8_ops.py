@@ -22,7 +22,7 @@ SIGNATURES = {
     "fg_kv8_write": [_P, _I, _P, _P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P,
                      _P, _P, _P, _I, _F, _I, _P],
     "fg_kv8_values": [_P, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _P, _P],
-    "fg_kv8_expand": [_P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P],
+    "fg_kv8_expand": [_P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _P, _P],
     "fg_kv8_attention_decode": [_P, _I, _P, _I, _P, _P, _I, _P, _P, _P, _I, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _F, _F, _P,
                                 _I, _P, _I, _P, _P, _P, _P],
     "fg_kv8_decode_scratch_floats": [],
@@ -240,7 +240,7 @@ class Kv8Ops:
             _ops._check(lib, lib.fg_kv8_expand(
                 _ops._ptr(memory.k_pages), _ops._ptr(memory.v_pages), _ops._ptr(memory.k_scales), _ops._ptr(memory.v_scales), _ops._ptr(table),
                 table.shape[1], _ops._ptr(ctx.seq_slot), _ops._ptr(ctx.seq_start), _ops._ptr(ctx.seq_cached), ctx.n_seqs, _ops._ptr(k), _ops._ptr(v), page,
-                n_pages, n_kv_heads, head_dim, signed_window, 0, _ops._ptr(self.status), _ops._stream()))
+                n_pages, n_kv_heads, head_dim, signed_window, _ops._ptr(self.status), _ops._stream()))
             expanded = dataclasses.replace(memory, k_pages=k, v_pages=v, k_scales=None, v_scales=None, tensor_maps=maps,
                                            layer_index=0)
             self.attention(q, out, expanded, _PromptsOnly(ctx), n_heads, n_kv_heads, head_dim, window, scale,

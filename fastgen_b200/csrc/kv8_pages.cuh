@@ -15,7 +15,7 @@ namespace fg_kv8 {
 //
 // Bound by latencies: a block is a chain of positions, pages, rows, angles and codes.  Steps of many tokens take stretches
 // of 64 tokens (PER = 4), a page of the usual size: with 16, three of four blocks found no run and left (2,048 prompt
-// tokens beside 20 single ones, 32 / 8 heads of 128: 34 us with one token a warp, 18 now).
+// tokens beside 20 single ones, 32 / 8 heads of 128, and their pages' values read back, 40 us; 23.9 now).
 // ---------------------------------------------------------------------------------
 constexpr int WRITE_WARPS = 16, WRITE_THREADS = 32 * WRITE_WARPS;
 constexpr int Q_SLICE = 8, Q_FLIGHT = 8;  // query heads a block rotates, and those whose rows are in flight together
@@ -474,10 +474,9 @@ __global__ void __launch_bounds__(EXPAND_THREADS)
 kv8_expand_kernel(const unsigned char* k_pages, const unsigned char* v_pages, const float* k_scales, const float* v_scales,
                   const int* __restrict__ block_table, int table_width, const int* __restrict__ seq_slot,
                   const int* __restrict__ seq_start, const int* __restrict__ seq_cached, int n_seqs, __nv_bfloat16* k_out,
-                  __nv_bfloat16* v_out, int page_size, int n_pages, int n_kv_heads, int window, int keep_first, int* status) {
+                  __nv_bfloat16* v_out, int page_size, int n_pages, int n_kv_heads, int window, int* status) {
   __shared__ int s_slot[EXPAND_THREADS], s_cached[EXPAND_THREADS], s_last[EXPAND_THREADS], s_n;
   pdl_trigger();
-  const int kept = (keep_first + page_size - 1) / page_size;
   const size_t bytes = (size_t)page_size * HD;
   const int grid = gridDim.x;
   bool waited = false;
@@ -507,15 +506,13 @@ kv8_expand_kernel(const unsigned char* k_pages, const unsigned char* v_pages, co
     for (int s = 0; s < s_n; ++s) {
       const int last = s_last[s];
       const int lo_page = first_visible(s_cached[s], window) / page_size;
-      const int n_kept = min(kept, lo_page);
-      const int items = (n_kept + last / page_size - lo_page + 1) * n_kv_heads * 2;
+      const int items = (last / page_size - lo_page + 1) * n_kv_heads * 2;
       // the blocks take the items of all sequences in turn
       const int first = ((int)blockIdx.x - before + grid) % grid;
       before = (before + items) % grid;
       for (int it = first; it < items; it += grid) {
         const bool is_v = it & 1;
-        const int g = (it >> 1) % n_kv_heads, i = (it >> 1) / n_kv_heads;
-        const int logical = i < n_kept ? i : lo_page + i - n_kept;
+        const int g = (it >> 1) % n_kv_heads, logical = lo_page + (it >> 1) / n_kv_heads;
         const int page = logical < table_width ? block_table[(size_t)s_slot[s] * table_width + logical] : -1;
         if (page < 0 || page >= n_pages) {
           if (status && threadIdx.x == 0) atomicOr(status, FG_STATUS_BAD_PAGE);

@@ -502,6 +502,25 @@ def test_attention_on_two_streams_and_in_graphs(ops):
     ops.check_status()
 
 
+def test_attention_right_behind_the_write_of_a_prompt(ops):
+    """A single token that reads what the launch before it wrote, all of it: the same with and without a pause between."""
+    size, page, heads, kv, n = 128, 64, 8, 8, 8000
+    cache = Cache(ops, 1, -(-n // page), kv, page, size)
+    g = torch.Generator().manual_seed(5)
+    q = torch.randn(1, heads * size, generator=g).to(torch.bfloat16).to(DEV)
+    ctx, out, want = _context([n - 1], [1]), torch.empty_like(q), torch.empty_like(q)
+    for _ in range(6):
+        k, v = ((torch.randn(n, kv * size, generator=g)).to(torch.bfloat16).to(DEV) for _ in range(2))
+        torch.cuda.synchronize()
+        cache.write(k, v, 0, 0)
+        ops.attention(q, out, cache.memory, ctx, heads, kv, size, None, 0.1)
+        torch.cuda.synchronize()
+        ops.attention(q, want, cache.memory, ctx, heads, kv, size, None, 0.1)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    ops.check_status()
+
+
 def test_bad_pages_are_reported(ops):
     from fastgen_b200.csrc.ops import KernelError
     size, page, heads, kv = 64, 64, 2, 1
