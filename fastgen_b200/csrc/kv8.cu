@@ -41,20 +41,22 @@ extern "C" int fg_kv8_write(const void* q, int q_stride, void* q_out, const void
                    ((2 * (long long)q_stride) % ALIGN) == 0 && ((2 * (long long)k_stride) % ALIGN) == 0 &&
                    ((2 * (long long)v_stride) % ALIGN) == 0;
   const int q_slices = (n_heads + Q_SLICE - 1) / Q_SLICE;
-  FG_CHECK_ARG(n_kv_heads + q_slices <= 65535, "fg_kv8_write: %d heads", n_heads);
-  auto launch = [&](auto kern, int per) {
+  auto launch = [&](auto kern, int per) -> int {
     const int stretch = WRITE_WARPS * per;
-    fg_launch_pdl(kern, dim3((n_tokens + stretch - 1) / stretch, n_kv_heads + q_slices), dim3(WRITE_THREADS), 0, stream,
+    const long long blocks = (long long)(n_tokens + stretch - 1) / stretch * n_kv_heads +
+                             (long long)(n_tokens + WRITE_WARPS - 1) / WRITE_WARPS * q_slices;
+    FG_CHECK_ARG(blocks < (1ll << 31), "fg_kv8_write: %d tokens of %d heads", n_tokens, n_heads);
+    fg_launch_pdl(kern, dim3((unsigned)blocks), dim3(WRITE_THREADS), 0, stream,
                   (const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)q_out, (const __nv_bfloat16*)k, k_stride,
                   (const __nv_bfloat16*)v, v_stride, pos, req, freqs, v_freqs, (unsigned char*)k_pages, (unsigned char*)v_pages,
                   k_scales, v_scales, block_table, table_width, page_size, n_pages, n_tokens, n_heads, n_kv_heads, status, rstd,
                   qn_w, kn_w, rstd_heads, magnitude, rot_pairs);
+    return 0;
   };
   // few tokens: a warp a token
-  if (n_tokens <= 512)
-    launch(vec ? kv8_write_kernel<FG_HEAD_DIM, true, 1> : kv8_write_kernel<FG_HEAD_DIM, false, 1>, 1);
-  else
-    launch(vec ? kv8_write_kernel<FG_HEAD_DIM, true, 4> : kv8_write_kernel<FG_HEAD_DIM, false, 4>, 4);
+  const int rc = n_tokens <= 512 ? launch(vec ? kv8_write_kernel<FG_HEAD_DIM, true, 1> : kv8_write_kernel<FG_HEAD_DIM, false, 1>, 1)
+                                 : launch(vec ? kv8_write_kernel<FG_HEAD_DIM, true, 4> : kv8_write_kernel<FG_HEAD_DIM, false, 4>, 4);
+  if (rc) return rc;
   FG_CHECK_LAUNCH("fg_kv8_write");
   return 0;
 }

@@ -13,9 +13,11 @@ namespace fg_kv8 {
 // the block's, a warp for four slots at a time, whose rows stay in registers between the search for the largest and the
 // rounding.  Blocks of the same stretch with higher indices rotate the queries.
 //
-// Bound by latencies: a block is a chain of positions, pages, rows, angles and codes.  Steps of many tokens take stretches
-// of 64 tokens (PER = 4), a page of the usual size: with 16, three of four blocks found no run and left (2,048 prompt
-// tokens beside 20 single ones, 32 / 8 heads of 128, and their pages' values read back, 40 us; 23.9 now).
+// Bound by instructions at many tokens (each key/value head's block computes the angles anew) and by latencies at few: a block is a
+// chain of positions, pages, rows, angles and codes.  Steps of many tokens take stretches of 64 tokens (PER = 4), a page of
+// the usual size: with 16, three of four blocks found no run and left.  Queries have blocks of their own, a warp a token.
+// (32 / 8 heads of 128: 2,048 prompt tokens beside 20 single ones 12.3 us, the write in 16 bits 9.4; 8,192 tokens 53.8 and 43.7.
+// With queries in the stretches' blocks and each thread looking through all places for the runs: 19.2 and 67.2.)
 // ---------------------------------------------------------------------------------
 constexpr int WRITE_WARPS = 16, WRITE_THREADS = 32 * WRITE_WARPS;
 constexpr int Q_SLICE = 8, Q_FLIGHT = 8;  // query heads a block rotates, and those whose rows are in flight together
@@ -65,8 +67,8 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
   __shared__ float s_amax[2][WRITE_WARPS];
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int t0 = blockIdx.x * STRETCH;
-  const int role = blockIdx.y;
+  // blocks of keys and values first, the heads of a stretch side by side; then those of queries
+  const int kv_blocks = (n_tokens + STRETCH - 1) / STRETCH * n_kv_heads;
 
   // sine and cosine of the lane's pairs at position p
   auto turns = [&](float (&sn)[E / 2], float (&cs)[E / 2], const float* table, int p, float mag) {
@@ -100,19 +102,15 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
     for (int i = 0; i < E; ++i) x[i] *= f * (w ? w[lane * E + i] : 1.f);
   };
 
-  if (role >= n_kv_heads) {
+  if ((int)blockIdx.x >= kv_blocks) {
     // ---- queries: a warp a token, the heads of the slice ----
-    const int h0 = (role - n_kv_heads) * Q_SLICE, h1 = min(n_heads, h0 + Q_SLICE);
-    bool waited = false;
-#pragma unroll 1
-    for (int u = 0; u < PER; ++u) {
-      const int t = t0 + warp * PER + u;
-      const int r = t < n_tokens ? req[t] : -1;
-      if (r < 0) continue;
-      float sn[E / 2], cs[E / 2];
-      turns(sn, cs, freqs, pos[t], magnitude);
-      if (!waited) pdl_wait();
-      waited = true;
+    const int slices = (n_heads + Q_SLICE - 1) / Q_SLICE, at = blockIdx.x - kv_blocks;
+    const int h0 = at % slices * Q_SLICE, h1 = min(n_heads, h0 + Q_SLICE), t = at / slices * WRITE_WARPS + warp;
+    const bool real = t < n_tokens && req[t] >= 0;
+    float sn[E / 2], cs[E / 2];
+    if (real) turns(sn, cs, freqs, pos[t], magnitude);
+    pdl_wait();
+    if (real) {
 #pragma unroll 1
       for (int hb = h0; hb < h1; hb += Q_FLIGHT) {
         uint32_t raw[Q_FLIGHT][E / 2];
@@ -142,12 +140,11 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
         }
       }
     }
-    if (!waited) pdl_wait();
     return;
   }
 
   // ---- keys and values of one head ----
-  const int g = role;
+  const int g = blockIdx.x % n_kv_heads, t0 = blockIdx.x / n_kv_heads * STRETCH;
   const __nv_bfloat16* const src[2] = {k + g * HD, v + g * HD};
   const int src_stride[2] = {k_stride, v_stride};
   unsigned char* const pool[2] = {k_pages, v_pages};
@@ -156,14 +153,21 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
 
   // the runs that begin at this warp's tokens: their lengths (0: none begins there) and pages
   bool any_long = false;
-#pragma unroll 1
+  const int mine = t0 + warp * PER;
+  int reqs[PER + 1], positions[PER + 1];  // of the token before the warp's, and of the warp's: all on their way together
+#pragma unroll
+  for (int u = 0; u <= PER; ++u) {
+    const int t = mine + u - 1;
+    const bool there = t >= 0 && t < n_tokens;
+    reqs[u] = there ? req[t] : -1;
+    positions[u] = there ? pos[t] : 0;
+  }
+#pragma unroll
   for (int u = 0; u < PER; ++u) {
-    const int t = t0 + warp * PER + u;
-    const int r = t < n_tokens ? req[t] : -1;
-    const int p = r >= 0 ? pos[t] : 0;
+    const int t = mine + u, r = reqs[u + 1], p = positions[u + 1];
     const int slot = p & (page_size - 1);
     int len = 0, page = -1;
-    if (r >= 0 && (t == 0 || slot == 0 || req[t - 1] != r || pos[t - 1] != p - 1)) {
+    if (r >= 0 && (slot == 0 || reqs[u] != r || positions[u] != p - 1)) {
       const int logical = p / page_size;
       page = logical < table_width ? block_table[(size_t)r * table_width + logical] : -1;
       const int most = min(page_size - slot, n_tokens - t);
@@ -192,16 +196,21 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
   any_long = __syncthreads_or(any_long);
   pdl_wait();
 
-  auto row_amax = [&](const float (&x)[E]) {
+  // The largest finite magnitude (fmaxf passes over NaNs); infinities become NaNs, as they are stored.
+  auto row_amax = [&](float (&x)[E]) {
     float a = 0.f;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const float m = fabsf(x[i]);
-      if (m <= 3.402823466e38f) a = fmaxf(a, m);  // neither infinities nor NaNs
+    for (int i = 0; i < E; ++i) a = fmaxf(a, fabsf(x[i]));
+    if (a == INFINITY) {
+      a = 0.f;
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        if (fabsf(x[i]) == INFINITY) x[i] = __int_as_float(0x7fffffff);
+        a = fmaxf(a, fabsf(x[i]));
+      }
     }
     return a;
   };
-  auto over = [&](float x, float f) { return fabsf(x) <= 3.402823466e38f ? x * f : __int_as_float(0x7fffffff); };
   // the page's exponent: from the run's largest magnitude and, behind cached entries, no lower than theirs
   auto exponents = [&](float amax, int slot, float before, int& old_e) {
     int e = scale_exponent(amax);
@@ -234,7 +243,7 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
     unsigned char* base = pool[kv] + block * (size_t)page_size * HD;
     uint32_t c[E / 2];
 #pragma unroll
-    for (int i = 0; i < E / 2; ++i) c[i] = codes_of(over(x[2 * i], inv), over(x[2 * i + 1], inv));
+    for (int i = 0; i < E / 2; ++i) c[i] = codes_of(x[2 * i] * inv, x[2 * i + 1] * inv);
     if (!kv) {
       unsigned char* dst = base + slot * HD + lane * E;
       if constexpr (E == 2) *reinterpret_cast<uint16_t*>(dst) = (uint16_t)c[0];
@@ -285,10 +294,17 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
   }
   if (!any_long) return;
 
+  unsigned todo = 0;  // runs of two and more tokens among 32 of the stretch's tokens
 #pragma unroll 1
-  for (int w = 0; w < STRETCH; ++w) {
+  for (int w = -1;;) {
+    todo &= todo - 1;
+    while (todo == 0 && (w | 31) + 1 < STRETCH) {
+      w = (w | 31) + 1;
+      todo = __ballot_sync(0xffffffffu, w + lane < STRETCH && s_len[(w + lane) % STRETCH] > 1);
+    }
+    if (todo == 0) break;
+    w = (w & ~31) + __ffs(todo) - 1;
     const int n = s_len[w];
-    if (n <= 1) continue;
     const int first = t0 + w, p0 = s_pos[w], slot = p0 & (page_size - 1);
     const size_t block = (size_t)s_page[w] * n_kv_heads + g;
     const float before[2] = {scale_before(0, block, slot), scale_before(1, block, slot)};
@@ -296,6 +312,7 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
     const int rounds = (page_size + 4 * WRITE_WARPS - 1) / (4 * WRITE_WARPS);
     uint32_t raw[2][4][E / 2];
     float x[4][E];  // keys, turned
+    float amax[2] = {0.f, 0.f};
     auto turned_v = [&](float (&y)[E], int i, int s) {
       unpacked(y, raw[1][i]);
       if (v_freqs != nullptr) {
@@ -303,6 +320,7 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
         turns(sn, cs, v_freqs, p0 + s - slot, 1.f);
         turn(y, sn, cs);
       }
+      return row_amax(y);
     };
     auto load_round = [&](int c) {
       const int s0 = 4 * (warp + WRITE_WARPS * c);
@@ -324,17 +342,15 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
         turns(sn, cs, freqs, p0 + s - slot, magnitude);
         normed(x[i], first + s - slot, n_heads + g, 1, norm_w);
         turn(x[i], sn, cs);
+        amax[0] = fmaxf(amax[0], row_amax(x[i]));
       }
     };
-    float amax[2] = {0.f, 0.f};
     for (int c = 0; c < rounds; ++c) {
       load_round(c);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        amax[0] = fmaxf(amax[0], row_amax(x[i]));
         float y[E];
-        turned_v(y, i, 4 * (warp + WRITE_WARPS * c) + i);
-        amax[1] = fmaxf(amax[1], row_amax(y));
+        amax[1] = fmaxf(amax[1], turned_v(y, i, 4 * (warp + WRITE_WARPS * c) + i));
       }
     }
     amax[0] = warp_max(amax[0]);
@@ -368,7 +384,7 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
         uint32_t wd[E];
 #pragma unroll
         for (int j = 0; j < E; ++j)
-          wd[j] = codes_of(over(x[0][j], inv[1]), over(x[1][j], inv[1])) | (codes_of(over(x[2][j], inv[1]), over(x[3][j], inv[1])) << 16);
+          wd[j] = codes_of(x[0][j] * inv[1], x[1][j] * inv[1]) | (codes_of(x[2][j] * inv[1], x[3][j] * inv[1]) << 16);
         if constexpr (E == 2) {
           *reinterpret_cast<uint2*>(dst) = make_uint2(wd[0], wd[1]);
         } else {
