@@ -94,7 +94,8 @@ class Kv8Ops:
         if (k.shape == shape and v.shape == (n_pages, n_kv_heads, page // 4, head_dim, 4) and ks.shape == scales == vs.shape
                 and k.dtype is v.dtype is _E4M3 and ks.dtype is vs.dtype is _F32 and k.is_contiguous() and v.is_contiguous()
                 and ks.is_contiguous() and vs.is_contiguous() and head_dim in build.KV8_HEAD_DIMS and page in _KV8_PAGES
-                and self.act_dtype is _BF16):
+                and self.act_dtype is _BF16 and k.device == v.device == ks.device == vs.device == memory.block_table.device
+                and k.is_cuda):
             return
         why = self.kv8_supported(head_dim, page)
         if why is not None:
@@ -104,6 +105,8 @@ class Kv8Ops:
         for t, dtype in ((k, _E4M3), (v, _E4M3), (ks, _F32), (vs, _F32)):
             if t.dtype != dtype or not t.is_contiguous():
                 raise ValueError(f"a cache in 8 bits: contiguous {dtype} wanted, got {t.dtype} {tuple(t.shape)}")
+        if not all(t.is_cuda and t.device == k.device for t in (k, v, ks, vs, memory.block_table)):
+            raise ValueError("a cache in 8 bits: its pages, scales and block table are on one GPU")
         raise ValueError(f"a cache in 8 bits of {n_kv_heads} heads of {head_dim}: keys {shape}, values "
                          f"{(n_pages, n_kv_heads, page // 4, head_dim, 4)} and scales {scales} wanted, got {tuple(k.shape)}, "
                          f"{tuple(v.shape)}, {tuple(ks.shape)} and {tuple(vs.shape)}")
@@ -138,9 +141,10 @@ class Kv8Ops:
         t = q.shape[0]
         kv_shape = (t, n_kv_heads * head_dim)
         if not (q.shape == (t, n_heads * head_dim) and k.shape == kv_shape == v.shape and q.dtype is k.dtype is v.dtype is _BF16
-                and q.stride(1) == k.stride(1) == v.stride(1) == 1 and n_heads % n_kv_heads == 0):
+                and q.stride(1) == k.stride(1) == v.stride(1) == 1 and n_heads % n_kv_heads == 0
+                and q.device == k.device == v.device == memory.k_pages.device):
             raise ValueError(f"rope_kv8_write takes bfloat16 rows of {n_heads} and twice {n_kv_heads} heads of {head_dim}, got "
-                             f"{q.dtype} {tuple(q.shape)}, {k.dtype} {tuple(k.shape)} and {v.dtype} {tuple(v.shape)}")
+                             f"{q.dtype} {tuple(q.shape)}, {k.dtype} {tuple(k.shape)} and {v.dtype} {tuple(v.shape)} on {q.device}")
         table = memory.block_table
         assert pos.dtype is req.dtype is table.dtype is torch.int32 and pos.numel() == req.numel() == t and table.is_contiguous()
         assert freqs is None or (freqs.dtype is _F32 and freqs.numel() == head_dim // 2 and freqs.is_contiguous())
@@ -168,7 +172,7 @@ class Kv8Ops:
         ``[n, kv heads, page, head size]``, every slot of the pages, also those that hold no token."""
         n_pages, n_kv_heads, page, head_dim = memory.k_pages.shape
         self._check_kv8(memory, n_kv_heads, head_dim)
-        assert pages.dtype is torch.int32 and pages.is_contiguous()
+        assert pages.dtype is torch.int32 and pages.is_contiguous() and pages.device == memory.k_pages.device
         n = pages.numel()
         k = torch.empty((n, n_kv_heads, page, head_dim), dtype=_BF16, device=pages.device)
         v = torch.empty_like(k)
@@ -223,8 +227,8 @@ class Kv8Ops:
     def _attention_kv8(self, q, out, memory, ctx, n_heads, n_kv_heads, head_dim, window, scale, out_freqs, keep_first,
                        softcap, sinks, chunk) -> bool:
         self._check_kv8(memory, n_kv_heads, head_dim)
-        assert q.dtype is out.dtype is _BF16 and q.stride(1) == 1 == out.stride(1)
-        assert not (window and chunk)
+        assert q.dtype is out.dtype is _BF16 and q.stride(1) == 1 == out.stride(1) and q.device == out.device == memory.k_pages.device
+        assert q.shape == out.shape and q.shape[1] == n_heads * head_dim and not (window and chunk)
         assert sinks is None or (sinks.dtype is _F32 and sinks.numel() == n_heads and sinks.is_contiguous())
         if window and keep_first:
             raise ValueError("a cache in 8 bits knows no window that keeps first positions")

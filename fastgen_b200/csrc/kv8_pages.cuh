@@ -11,7 +11,7 @@ namespace fg_kv8 {
 // work of one block, found on the device: a block looks at a stretch of tokens, PER a warp, and takes the runs that begin
 // among them, keys and values of one key/value head.  A run of one token (a decoded token) is a warp's work; a longer run is
 // the block's, a warp for four slots at a time, whose rows stay in registers between the search for the largest and the
-// rounding.  Blocks of the same stretch with higher indices rotate the queries.
+// rounding.
 //
 // Bound by instructions at many tokens (each key/value head's block computes the angles anew) and by latencies at few: a block is a
 // chain of positions, pages, rows, angles and codes.  Steps of many tokens take stretches of 64 tokens (PER = 4), a page of
@@ -169,7 +169,7 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
     int len = 0, page = -1;
     if (r >= 0 && (slot == 0 || reqs[u] != r || positions[u] != p - 1)) {
       const int logical = p / page_size;
-      page = logical < table_width ? block_table[(size_t)r * table_width + logical] : -1;
+      page = p >= 0 && logical < table_width ? block_table[(size_t)r * table_width + logical] : -1;
       const int most = min(page_size - slot, n_tokens - t);
       for (int at = 0; at < most; at += 32) {
         const int i = at + lane;

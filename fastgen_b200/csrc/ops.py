@@ -1121,8 +1121,8 @@ class Ops(Kv8Ops):
         n = w.rows
         if x.dtype is not _BF16 or self.act_dtype is not _BF16:
             raise ValueError(f"4-bit weights take bfloat16 activations, got {x.dtype}")
-        if w.columns != k or x.stride(1) != 1:
-            raise ValueError(f"a product of {tuple(x.shape)} with 4-bit weights {w.shape}")
+        if w.columns != k or x.stride(1) != 1 or w.device != x.device:
+            raise ValueError(f"a product of {tuple(x.shape)} on {x.device} with 4-bit weights {w.shape} on {w.device}")
         if bias is not None and (bias.shape != (n,) or bias.dtype is not _BF16 or not bias.is_contiguous()):
             raise ValueError(f"the bias of {n} rows is contiguous bfloat16, got {bias.dtype} {tuple(bias.shape)}")
         if m >= W4_DENSE_M:
@@ -1133,8 +1133,8 @@ class Ops(Kv8Ops):
                 return self.linear(x, dense, out=out, out_dtype=out_dtype, bias=bias, act=act)
             return self.silu_gate(self.linear(x, dense), torch.empty((m, n // 2), dtype=_BF16, device=x.device), 8, act=act or "silu")
         ldx, at = x.stride(0), x.data_ptr()
-        if ldx % 8 or at % 16:
-            x = torch.empty((m, k), dtype=_BF16, device=x.device).copy_(x)  # rows off 16 bytes (k is a multiple of 32)
+        if ldx % 8 or at % 16 or ldx < k:
+            x = torch.empty((m, k), dtype=_BF16, device=x.device).copy_(x)  # rows off 16 bytes, or one row for all of them
             ldx, at = x.stride(0), x.data_ptr()
         if out is None:
             out = torch.empty((m, n // 2 if gated else n), dtype=out_dtype or _BF16, device=x.device)

@@ -38,7 +38,7 @@ class Weight4:
     @staticmethod
     def _packed(codes: torch.Tensor) -> torch.Tensor:
         n, half = codes.shape
-        four = codes.view(n, half // 4, 4)  # bytes of eight columns: even columns low, odd ones high
+        four = codes.reshape(n, half // 4, 4)  # bytes of eight columns: even columns low, odd ones high
         even, odd = four & 15, four >> 4
         pairs = torch.stack([even, odd], dim=2)  # [n, words, 2, 4]: the low half's nibbles, then the high half's
         out = pairs[..., 0::2] | (pairs[..., 1::2] << 4)  # [n, words, 2, 2]

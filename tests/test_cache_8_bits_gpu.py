@@ -538,9 +538,10 @@ def test_bad_pages_are_reported(ops):
     _check(out[1:], want, room)
     x = torch.zeros(3, kv * size, dtype=torch.bfloat16, device=DEV)
     before = cache.memory.k_pages.view(torch.uint8).clone()
-    cache.write(x, x, 0, 70)
-    with pytest.raises(KernelError, match="block-table entry"):
-        ops.check_status()
+    for start in (70, -5, -500):  # a page that is not there, positions that are none
+        cache.write(x, x, 0, start)
+        with pytest.raises(KernelError, match="block-table entry"):
+            ops.check_status()
     assert torch.equal(before, cache.memory.k_pages.view(torch.uint8))
 
 
@@ -562,6 +563,13 @@ def test_refusals(ops):
         ops.rope_kv8_write(q, k, k, at, at, None, replace(mem, k_scales=mem.k_scales[:1]), 4, 2, 64)
     with pytest.raises(ValueError, match="wanted, got"):
         ops.attention(q, q.clone(), replace(mem, v_pages=mem.k_pages), ctx, 4, 2, 64, None, 1.0)
+    for field in ("k_pages", "v_pages", "k_scales", "v_scales", "block_table"):
+        with pytest.raises(ValueError, match="on one GPU"):
+            ops.attention(q, q.clone(), replace(mem, **{field: getattr(mem, field).cpu()}), ctx, 4, 2, 64, None, 1.0)
+    with pytest.raises(ValueError, match="bfloat16 rows"):
+        ops.rope_kv8_write(q.cpu(), k, k, at, at, None, mem, 4, 2, 64)
+    with pytest.raises(AssertionError):
+        ops.attention(q[:, :128], q.clone(), mem, ctx, 4, 2, 64, None, 1.0)
     with pytest.raises(ValueError, match="keeps first positions"):
         ops.attention(q, q.clone(), mem, ctx, 4, 2, 64, 10, 1.0, keep_first=4)
     with pytest.raises(ValueError, match="serves bfloat16"):

@@ -28,6 +28,14 @@ def test_weights_of_4_bits_stand_for_what_they_say():
         assert w.nbytes() == 7 * 192 + 2 * scales.numel()
 
 
+def test_codes_may_be_a_view():
+    from fastgen_b200.weights import Weight4
+    g = torch.Generator().manual_seed(3)
+    codes = torch.randint(0, 256, (64, 6), dtype=torch.uint8, generator=g).t()  # [6, 64], columns neighbours in memory
+    scales = torch.rand(2, 6, generator=g).bfloat16().t()
+    assert torch.equal(Weight4(codes, scales).dequantize(), Weight4(codes.contiguous(), scales.contiguous()).dequantize())
+
+
 @pytest.mark.parametrize("group", [32, 64, 128])
 def test_quantized_weights_are_the_nearest(group):
     """Half a step of the scale, and what rounding the scale to bfloat16 (2^-8 of it) leaves at the ends, 7 steps away."""
@@ -166,6 +174,49 @@ def test_models_with_a_cache_in_8_bits(tmp_path, name, page):
                     worst = max(worst, off)
                     assert off <= 2.0 ** -4, (plan, rid, p, off)
     print(f"worst row {worst:.4f}")
+
+
+def _pegurax():
+    import test_pegurax_gpu as m
+    return m, "pc", (m.T_L2, 0.0, 1.0)  # pairs whose attention has chunks, head sizes 64 and 128 in one model
+
+
+def _palulorn():
+    import test_palulorn_gpu as m
+    layers = [m._layer("attention", m._attn(6, 3, 64, 32, 0.1, conv=2, rot=(8, 5000.0, 8.0), window=20), m._moe(6, 3, 40, (3, 2), 2.0, 24)),
+              m._layer("parallel", m._pair(m._sink(4, 2, 64, 0.15, (0.5, 7)), m._memory(3, 24, 40, 10.0)), m._moe(5, 2, 24)),
+              m._layer("attention", m._attn(2, 1, 128, 48, 0.12, conv=4, rot=(24, 300.0, None), window=70), None)]
+    m.CONFIGS["fewer bits"] = (dict(architecture="Palulorn", vocab=211, width=96, norm=dict(eps=1e-5), embedding=dict(scale=3.0),
+                                    loop=dict(start=1, stop=3, times=2), layers=layers), 21)
+    return m, "fewer bits", (m.T_L2, m.T_SHARE, m.T_FAR)  # sinks, values that are keys, windows, convolutions, layers passed twice
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("design", [_pegurax, _palulorn])
+def test_other_designs_with_a_cache_in_8_bits(tmp_path, design):
+    """Mixers that join attention with others, through the engine, held to that design's own bfloat16 rule widened by the
+    entries' rounding: an entry is off by 2^-4 of itself at most, so attention's outputs are off by 2^-4 of the largest value
+    where bfloat16 has them off by its 2^-8, and what the design's rule allows a row (``T_L2`` of its norm) grows by 2^-4.
+    Where the rule lets a share of the rows be ``T_FAR`` times as far, because a read-out that nearly cancels carries what
+    comes in at full size, that factor is on both.  On average, where roundings are random, rows are within half."""
+    m, name, (room, share, far_times) = design()
+    room += 2.0 ** -4
+    folder = m.model_dir(tmp_path, name, torch.bfloat16)
+    vocab = m.CONFIGS[name][0]["vocab"]
+    requests = _requests(vocab, [150, 3, 77, 200], 5)
+    steps = H.plan_mixed(requests, 3)
+    for graphs in (True, False):
+        out, engine = _run(folder, steps, 32, H.max_live_tokens(steps, 64) + 512, cache_bits=8, graphs=graphs,
+                           max_step_tokens=256 if graphs else None)
+        assert all(g.k_pages.dtype == torch.float8_e4m3fn for g in engine.cache.groups)
+        got = H.collect(steps, out)
+        far = []
+        for rid, tokens in requests.items():
+            want = m.plain_logits(folder, tokens)
+            far += [float(np.linalg.norm(row - want[p]) / np.linalg.norm(want[p])) for p, row in got[rid].items()]
+        print(f"worst row {max(far):.4f}, average {np.mean(far):.4f}")
+        assert max(far) <= far_times * room and np.mean(far) <= room / 2
+        assert sum(x > room for x in far) <= share * len(far)
 
 
 @pytest.mark.gpu

@@ -108,6 +108,17 @@ def test_rows_and_special_numbers(ops):
     assert ops.linear(x[:0], w).shape == (0, 300)
 
 
+@pytest.mark.parametrize("m", [3, 20])
+def test_one_row_for_all_tokens_and_the_same_twice(ops, m):
+    """Rows without a stride between them; two calls with the same operands."""
+    g = torch.Generator().manual_seed(m)
+    w = _weight(g, 130, 256, 64)
+    row = torch.randn(1, 256, generator=g).to(torch.bfloat16).to(DEV)
+    y = ops.linear(row.expand(m, -1), w)
+    assert torch.equal(y, ops.linear(row.repeat(m, 1), w)) and torch.equal(y, ops.linear(row.expand(m, -1), w))
+    assert ops.linear(row[:0], w).shape == (0, 130)
+
+
 def test_two_products_at_once_and_in_a_graph(ops):
     """Clusters of two launches side by side on the chip; a captured product gives the eager one's bits."""
     g = torch.Generator().manual_seed(5)
@@ -138,6 +149,9 @@ def test_refusals(ops):
     from fastgen_b200.csrc.ops import Ops
     g = torch.Generator().manual_seed(0)
     w = _weight(g, 40, 128, 64)
+    for m in (1, 20, 300):
+        with pytest.raises(ValueError, match="on cpu"):
+            ops.linear(torch.zeros(m, 128, dtype=torch.bfloat16), w)
     x = torch.zeros(2, 128, dtype=torch.bfloat16, device=DEV)
     with pytest.raises(ValueError, match="bfloat16 activations"):
         ops.linear(x.float(), w)
