@@ -30,6 +30,8 @@
 
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "attention_mma.cuh"
 #include "kv8.cuh"
 
@@ -638,19 +640,20 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
       const int g = s_run[x][1] / n_sub, sub = s_run[x][1] - g * n_sub;
       const int heads = min(MAX_COLUMNS, group - sub * MAX_COLUMNS), head0 = g * group + sub * MAX_COLUMNS;
       __nv_bfloat16* const dst = out + (size_t)s_run[x][2] * out_stride + head0 * HD;
-      // every partial of this request and head is there: a thread merges four neighbouring dimensions of a head, eight
-      // partials' loads in flight together
+      // every partial of this request and head is there: a thread merges four neighbouring dimensions of a head, the
+      // loads of sixteen partials in flight together, of eight where no more are left
       for (int y = tid; y < heads * (HD / 4); y += CONSUMERS) {
         const int r = y / (HD / 4), d = 4 * (y - r * (HD / 4));
         float m = -INFINITY, l = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int b0 = first_block; b0 <= last_block; b0 += 8) {
-          float2 ml[8];
-          float4 v[8];
+        auto merged = [&](auto flight, int b0) {
+          constexpr int FLIGHT = decltype(flight)::value;
+          float2 ml[FLIGHT];
+          float4 v[FLIGHT];
 #pragma unroll
-          for (int u = 0; u < 8; ++u) {
+          for (int u = 0; u < FLIGHT; ++u) {
             const int b = b0 + u;
             const float* from = scratch + (((size_t)min(b, last_block) * 2 + (b == first_block)) * MAX_COLUMNS + r) * run_stride<HD>();
-            // (volatile: all sixteen leave before the first is waited for)
+            // (volatile: all of them leave before the first is waited for)
             asm volatile("ld.global.cg.v2.f32 {%0,%1}, [%2];\n" : "=f"(ml[u].x), "=f"(ml[u].y) : "l"(from + HD) : "memory");
             asm volatile("ld.global.cg.v4.f32 {%0,%1,%2,%3}, [%4];\n"
                          : "=f"(v[u].x), "=f"(v[u].y), "=f"(v[u].z), "=f"(v[u].w)
@@ -659,7 +662,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
           }
           float top = m;
 #pragma unroll
-          for (int u = 0; u < 8; ++u) {
+          for (int u = 0; u < FLIGHT; ++u) {
             if (b0 + u > last_block) ml[u] = make_float2(-INFINITY, 0.f);  // (the last one once more: nothing)
             top = fmaxf(top, ml[u].x);
           }
@@ -669,13 +672,22 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
 #pragma unroll
           for (int e = 0; e < 4; ++e) a[e] *= keep;
 #pragma unroll
-          for (int u = 0; u < 8; ++u) {
+          for (int u = 0; u < FLIGHT; ++u) {
             const float f = ml[u].x == -INFINITY ? 0.f : ex2(ml[u].x - top);
             l += f * ml[u].y;
             a[0] += f * v[u].x;
             a[1] += f * v[u].y;
             a[2] += f * v[u].z;
             a[3] += f * v[u].w;
+          }
+        };
+        for (int b0 = first_block; b0 <= last_block;) {
+          if (last_block - b0 >= 8) {
+            merged(std::integral_constant<int, 16>(), b0);
+            b0 += 16;
+          } else {
+            merged(std::integral_constant<int, 8>(), b0);
+            b0 += 8;
           }
         }
         const float f = finish(m, l, sinks, head0 + r);
