@@ -457,6 +457,56 @@ def test_prompt_portions(ops, size, page, heads, kv, option):
     _check(out, want, 2 * room)
 
 
+@pytest.mark.parametrize("size,page", [(64, 16), (64, 64), (128, 32), (128, 128), (128, 256), (256, 16)])
+@pytest.mark.parametrize("option", ["plain", "window", "chunk"])
+def test_pages_that_were_given_back(ops, size, page, option):
+    """Pages that no later query sees are gone from the table and hold other sequences' NaNs, as does the pool that portions read."""
+    kv, heads = 2, 4
+    cached, new = [0, 700, 300, 513, 640], [150, 40, 1, 2, 1]
+    cache = Cache(ops, len(new), -(-760 // page) + 1, kv, page, size)
+    for s, (c, n) in enumerate(zip(cached, new)):
+        cache.fill(s, c + n, s + size)
+    args = dict(window=dict(window=100), chunk=dict(chunk=192), plain={})[option]
+    ctx = _context(cached, new)
+    g = torch.Generator().manual_seed(page)
+    q = torch.randn(sum(new), heads * size, generator=g).to(torch.bfloat16).to(DEV)
+    want, room = _attention(cache, q, ctx, heads, size ** -0.5, **args)
+    for s, c in enumerate(cached):
+        first = max(0, c + 1 - 100) if option == "window" else c // 192 * 192 if option == "chunk" else 0
+        for logical in range(first // page):
+            at = int(cache.table[s, logical])
+            for pool in (cache.memory.k_pages, cache.memory.v_pages):
+                pool.view(torch.uint8)[at] = 0x7F
+            cache.table[s, logical] = -1
+    for pool in ops.kv8_expanded(cache.memory)[:2]:
+        pool.fill_(float("nan"))
+    out = torch.empty_like(q)
+    call = dict(args)
+    window = call.pop("window", None)
+    ops.attention(q, out, cache.memory, ctx, heads, kv, size, window, size ** -0.5, **call)
+    ops.check_status()
+    _check(out, want, 2 * room)
+
+
+def test_the_first_call_is_not_captured(ops):
+    """Work buffers are made outside a capture; what needs them inside one is refused, and served after a first call."""
+    from fastgen_b200.csrc.ops import Ops
+    size, page, heads, kv = 64, 32, 4, 2
+    cache = Cache(ops, 2, 8, kv, page, size)
+    for s in range(2):
+        cache.fill(s, 200, s)
+    fresh = Ops(torch.bfloat16, DEV)
+    for ctx in (_context([199], [1]), _context([150], [50])):
+        q = torch.randn(ctx.n_tokens, heads * size, device=DEV).to(torch.bfloat16)
+        out, want = torch.zeros_like(q), torch.zeros_like(q)
+        ops.attention(q, want, cache.memory, ctx, heads, kv, size, None, 0.1)
+        with pytest.raises(RuntimeError, match="graph capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                fresh.attention(q, out, cache.memory, ctx, heads, kv, size, None, 0.1)
+        fresh.attention(q, out, cache.memory, ctx, heads, kv, size, None, 0.1)
+        assert torch.equal(out, want)
+
+
 def test_attention_on_two_streams_and_in_graphs(ops):
     """A call on another stream is ordered behind the first; a captured call gives the eager one's bits, for other lengths than
     it was captured with, too."""
