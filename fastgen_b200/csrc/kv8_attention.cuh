@@ -39,7 +39,6 @@ namespace fg_kv8 {
 
 using fg_mma::capped_score;
 using fg_mma::mbar_arrive;
-using fg_mma::mbar_arrive_expect;
 using fg_mma::mbar_fence_init;
 using fg_mma::mbar_init;
 using fg_mma::mbar_wait;
@@ -72,6 +71,11 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
           smem_u32(dst)),
       "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
       : "memory");
+}
+
+// bytes that a barrier's phase waits for, without an arrival
+__device__ __forceinline__ void mbar_expect(uint64_t* bar, int bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;\n" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -280,24 +284,14 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
       const int k0 = (w.first + w.split) * SPLIT, g = w.slice / n_sub;
       const size_t block = (size_t)max(page, 0) * n_kv_heads + g;
       const uint32_t ks = page >= 0 ? ld_global_4(k_scales + block) : 0u, vs = page >= 0 ? ld_global_4(v_scales + block) : 0u;
-      // the next item's pages are on their way meanwhile
-      int next_page = -1;
-      if (i + 1 < count) {
-        advance(w);
-        next_page = page_of(w);
-      }
       const unsigned valid = __ballot_sync(0xffffffffu, page >= 0);
       const int bytes = __popc(valid) * box_rows * HD;
       const int line0 = (k0 & (page_size - 1)) * HD / 128;  // 0 unless pages are longer than a split
+      const int k_slot = slot;
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
         if (use > 0) mbar_wait(&empty[slot], (use - 1) & 1, status, &gave_up);
-        if (kv == 0 && lane < n_boxes) {
-          s_exp[slot][0][lane] = page >= 0 ? exponent_of_scale(__uint_as_float(ks)) : NO_PAGE;
-          s_exp[slot][1][lane] = page >= 0 ? exponent_of_scale(__uint_as_float(vs)) : 0;
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive_expect(&full[slot], bytes);
+        if (lane == 0) mbar_expect(&full[slot], bytes);
         __syncwarp();
         if (page >= 0)  // lane i issues box i's copy
           tma_load_3d(ring + slot * SLOT_BYTES + lane * box_rows * HD, kv ? &v_map : &k_map, 0, line0,
@@ -307,8 +301,26 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
           ++use;
         }
       }
+      // the next item's pages and the scales come while the copies run; consumers read the scales behind the keys' arrival
+      int next_page = -1;
+      if (i + 1 < count) {
+        advance(w);
+        next_page = page_of(w);
+      }
+      if (lane < n_boxes) {
+        s_exp[k_slot][0][lane] = page >= 0 ? exponent_of_scale(__uint_as_float(ks)) : NO_PAGE;
+        s_exp[k_slot][1][lane] = page >= 0 ? exponent_of_scale(__uint_as_float(vs)) : 0;
+      }
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&full[k_slot]);
+        mbar_arrive(&full[k_slot + 1 == SLOTS ? 0 : k_slot + 1]);
+      }
       page = next_page;
     }
+    if (*reinterpret_cast<volatile int*>(&gave_up) != 0)
+      // a wait ran out: the copies in flight land before the block leaves
+      for (int f = max(0, 2 * count - SLOTS); f < 2 * count; ++f) mbar_wait(&full[f % SLOTS], f / SLOTS & 1, status);
   } else {
     // ================================ consumers ================================
     pdl_wait();
