@@ -136,7 +136,8 @@ class Kv8Ops:
         (``e >= -100``) at which every magnitude is at most ``448 * 2^e``.  Tokens that begin a page choose it; tokens
         behind cached ones never lower it, and where they raise it the cached codes are rounded again.  A sequence's
         tokens are neighbours in the step and in ascending order.  Entries that are not finite are stored as NaN.
-        Queries, keys and values are bfloat16; the rotated numbers are rounded once, to their codes."""
+        Queries, keys and values are bfloat16; the rotated numbers are rounded once, to the
+        codes nearest to their values in 64 bits (of the float32 angle position * frequency)."""
         self._check_kv8(memory, n_kv_heads, head_dim)
         t = q.shape[0]
         kv_shape = (t, n_kv_heads * head_dim)

@@ -16,8 +16,9 @@ namespace fg_kv8 {
 // Bound by instructions at many tokens (each key/value head's block computes the angles anew) and by latencies at few: a block is a
 // chain of positions, pages, rows, angles and codes.  Steps of many tokens take stretches of 64 tokens (PER = 4), a page of
 // the usual size: with 16, three of four blocks found no run and left.  Queries have blocks of their own, a warp a token.
-// (32 / 8 heads of 128: 2,048 prompt tokens beside 20 single ones 12.3 us, the write in 16 bits 9.4; 8,192 tokens 53.8 and 43.7.
-// With queries in the stretches' blocks and each thread looking through all places for the runs: 19.2 and 67.2.)
+// (32 / 8 heads of 128: 2,048 prompt tokens beside 20 single ones 14.2 us, the write in 16 bits 9.4; 8,192 tokens 65.7 and 43.7.
+// Before codes in doubt were settled in 64 bits: 12.3 and 53.8; with queries in the stretches' blocks and each thread looking
+// through all places for the runs: 19.2 and 67.2.)
 // ---------------------------------------------------------------------------------
 constexpr int WRITE_WARPS = 16, WRITE_THREADS = 32 * WRITE_WARPS;
 constexpr int Q_SLICE = 8, Q_FLIGHT = 8;  // query heads a block rotates, and those whose rows are in flight together
@@ -51,6 +52,21 @@ __device__ __forceinline__ void unpacked(float (&x)[E], const uint32_t (&w)[E / 
     x[2 * i] = __uint_as_float(w[i] << 16);
     x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
   }
+}
+
+// A turned pair in 64 bits, for numbers whose code the float32 ones leave in doubt (one in some 40,000, and exact ties): w0 and w1
+// are the norm's factors, the angle is float32 by definition.  To float32 with the last bit set where bits are lost, so that
+// the rounding to a code is the only one.
+__device__ __noinline__ float2 turned_exactly(const __nv_bfloat16* at, double w0, double w1, float angle, float magnitude) {
+  const volatile unsigned short* raw = reinterpret_cast<const volatile unsigned short*>(at);
+  const double a = (double)__uint_as_float((uint32_t)raw[0] << 16) * w0, b = (double)__uint_as_float((uint32_t)raw[1] << 16) * w1;
+  double sn, cs;
+  sincos((double)angle, &sn, &cs);
+  auto narrowed = [](double x) {
+    const float r = __double2float_rz(x);
+    return (double)r == x ? r : __uint_as_float(__float_as_uint(r) | 1u);
+  };
+  return make_float2(narrowed((a * cs - b * sn) * magnitude), narrowed((b * cs + a * sn) * magnitude));
 }
 
 template <int HD, bool VEC, int PER>
@@ -258,6 +274,34 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
       }
     }
   };
+  // Turned numbers are off by less than 2^-21 of their pair's magnitudes (sine and cosine 2^-23, two products and a sum 2^-24
+  // each, and the square root of two from a pair to its turn), with a norm's factors or a magnitude less than 2^-20.  Where that
+  // could change a code, and something has been rounded at all, the pair is computed in 64 bits.  (Without this one code in a
+  // million is the neighbouring one; it takes 2 of the 14 us given above; doubts kept in a list and
+  // settled behind the run 3.)
+  const bool turned[2] = {freqs != nullptr || rstd != nullptr, v_freqs != nullptr};  // else the numbers are exact
+  const float off = rstd != nullptr || magnitude != 1.f ? 0x1p-20f : 0x1p-21f;
+  auto settled = [&](int kv, float (&x)[E], int t, int p, float inv) {
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+      const float y0 = x[2 * i] * inv, y1 = x[2 * i + 1] * inv, d = (fabsf(y0) + fabsf(y1)) * off;
+      if (d != 0.f && codes_of(y0 - d, y1 - d) != codes_of(y0 + d, y1 + d)) {
+        const float* table = kv ? v_freqs : freqs;
+        const int j = lane * (E / 2) + i;
+        const float angle = table ? (float)p * table[j] : 0.f, factor = table && !kv && j < rot_pairs ? magnitude : 1.f;
+        const bool normed_too = !kv && rstd != nullptr;
+        if (angle == 0.f && factor == 1.f && !normed_too) continue;
+        double w0 = 1.0, w1 = 1.0;
+        if (normed_too) {
+          w0 = w1 = rstd_heads ? rstd[(size_t)t * rstd_heads + n_heads + g] : rstd[2 * (size_t)t + 1];
+          if (norm_w) w0 *= norm_w[2 * j], w1 *= norm_w[2 * j + 1];
+        }
+        const float2 v = turned_exactly(src[kv] + (size_t)t * src_stride[kv] + 2 * j, w0, w1, angle, factor);
+        x[2 * i] = v.x;
+        x[2 * i + 1] = v.y;
+      }
+    }
+  };
   auto scale_before = [&](int kv, size_t block, int slot) {
     return slot > 0 ? __uint_as_float(ld_global_4(scales[kv] + block)) : 1.f;
   };
@@ -288,6 +332,7 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
         rescale(kv, block, slot, exp2_int(max(old_e - e, -126)), lane, 32);
         __syncwarp();
       }
+      if (turned[kv]) settled(kv, x, t, p, exp2_int(-e));
       store_row(kv, x, block, slot, exp2_int(-e));
       if (lane == 0 && (slot == 0 || e > old_e)) scales[kv][block] = exp2_int(e);
     }
@@ -375,9 +420,16 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
       const int s0 = 4 * (warp + WRITE_WARPS * c);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (s0 + i >= slot && s0 + i < slot + n) store_row(0, x[i], block, s0 + i, inv[0]);
+        if (s0 + i >= slot && s0 + i < slot + n) {
+          if (turned[0]) settled(0, x[i], first + s0 + i - slot, p0 + s0 + i - slot, inv[0]);
+          store_row(0, x[i], block, s0 + i, inv[0]);
+        }
 #pragma unroll
       for (int i = 0; i < 4; ++i) turned_v(x[i], i, s0 + i);  // now the values
+      if (turned[1])
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (s0 + i >= slot && s0 + i < slot + n) settled(1, x[i], first + s0 + i - slot, p0 + s0 + i - slot, inv[1]);
       if (s0 >= slot && s0 + 4 <= slot + n) {
         // a whole group of four tokens: words
         uint32_t* dst = reinterpret_cast<uint32_t*>(v_pages + block * (size_t)page_size * HD + (size_t)s0 * HD) + lane * E;

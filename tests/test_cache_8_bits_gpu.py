@@ -216,6 +216,49 @@ def test_write_of_mixed_steps(ops, size, page, heads, kv, option):
         assert torch.equal(old_v[:, used:], new_v[:, used:])
 
 
+@pytest.mark.parametrize("size,option", [(64, "plain"), (128, "plain"), (256, "plain"), (128, "values turned"), (128, "norm a token"), (64, "norm a head"),
+                                         (128, "every pair in doubt"), (64, "half turned")])
+def test_codes_are_the_nearest_in_64_bits(ops, size, option):
+    """Four million turned numbers, of a prompt and of single tokens: each has the code of its 64-bit value.  (Float32 alone puts
+    one in a million next to a border on the wrong side.)"""
+    page, kv, t = 64, 8, 4096 * 128 // size
+    g = torch.Generator().manual_seed(size)
+    cache = Cache(ops, 64, -(-t // page), kv, page, size)
+    k, v = ((torch.randn(t, kv * size, generator=g)).to(torch.bfloat16).to(DEV) for _ in range(2))
+    freqs = (10000.0 ** (-torch.arange(size // 2) / (size // 2))).float().to(DEV)
+    rstd = weights = None
+    if option == "every pair in doubt":
+        # numbers that lie between two codes before they are turned by next to nothing
+        freqs.fill_(2.0 ** -40)
+        k = ((torch.randint(8, 16, k.shape, generator=g) + 0.5) * 2.0).to(torch.bfloat16).to(DEV)
+    elif option == "half turned":
+        freqs[size // 4 :] = 0
+    if option == "norm a token":
+        rstd, weights = torch.rand(t, 2, generator=g).to(DEV) + 0.5, torch.rand(kv * size, generator=g).to(DEV) + 0.5
+    elif option == "norm a head":
+        rstd, weights = torch.rand(t, 2 * kv, generator=g).to(DEV) + 0.5, torch.rand(kv * size, generator=g).to(DEV) + 0.5
+    options = dict(v_freqs=freqs if option == "values turned" else None, qk_norm=None if rstd is None else (rstd, weights, weights))
+    q = torch.zeros(t, kv * size, dtype=torch.bfloat16, device=DEV)
+    singles = torch.arange(60, dtype=torch.int32, device=DEV)
+    for pos, req in ((torch.arange(t, dtype=torch.int32, device=DEV), torch.full((t,), 63, dtype=torch.int32, device=DEV)), (singles % 30 * page, singles)):
+        n = pos.numel()
+        wide = dict(options, qk_norm=None if rstd is None else (rstd[:n].contiguous(), weights, weights))
+        ops.rope_kv8_write(q[:n], k[:n], v[:n], pos, req, freqs, cache.memory, kv, kv, size, **wide)
+        x = k[:n].double().view(n, kv, size)
+        if rstd is not None:
+            x = x * (rstd[:n, 1:2] if rstd.shape[1] == 2 else rstd[:n, kv:]).double()[:, :, None] * weights.double().view(kv, size)
+        x, y = _turned(x, pos, freqs), v[:n].double().view(n, kv, size)
+        if option == "values turned":
+            y = _turned(y, pos, freqs)
+        at = cache.table[req.long(), (pos // page).long()].long()
+        mem = cache.memory
+        kc = cache.values[mem.k_pages.view(torch.uint8)[at, :, (pos % page).long()].long()]
+        vc = cache.values[mem.v_pages.view(torch.uint8)[at, :, (pos % page // 4).long(), :, (pos % 4).long()].long()]
+        assert torch.equal(kc, _nearest(x / mem.k_scales[at].double()[..., None]))
+        assert torch.equal(vc, _nearest(y / mem.v_scales[at].double()[..., None]))
+    ops.check_status()
+
+
 @pytest.mark.parametrize("size", [64, 128])
 def test_write_of_unusual_numbers(ops, size):
     """Zeros, the ends of bfloat16's range, infinities and NaN: the others of the page keep their scale and their codes."""
