@@ -19,7 +19,9 @@
 //    score the weight of the second product is 2^(s + f - m), m the largest s + f, so that weights stay within half
 //    precision whatever the pages' scales are, and the codes enter the product as they are.  The softmax's denominator is
 //    the sum of 2^(s - m), taken apart.  Weights are held 2^15 times larger than their value (half precision then
-//    reaches down to 2^-39 of the largest).
+//    reaches down to 2^-39 of the largest); the denominator is not, for it lies between 2^-100 and 2^100 times the number
+//    of keys (a value's scale is 2^-100 at the least and 2^100 at the most), within float32 for up to 2^27 keys.  Where scales
+//    lie far apart, what brings a denominator to a new maximum is applied in two halves: 2^100 times 2^-200 is 2^-100.
 //  * A value word holds the codes of four neighbouring keys of one dimension, so that a conversion gives the pairs of keys
 //    that an operand register wants.  Keys are dealt to the rows of the first product such that its result, transposed in
 //    registers, has the same order: row r < 8 of a tile of 16 keys is key 4 (r / 2) + r % 2, row r + 8 that key + 2.
@@ -49,7 +51,9 @@ constexpr int DECODE_THREADS = 160;          // 4 consumer warps + 1 producer wa
 constexpr int CONSUMERS = 128;
 constexpr int MAX_COLUMNS = 8;       // heads of a group that an item works on
 constexpr int DECODE_MAX_SEQS = 4096;
-constexpr float WEIGHT_SHIFT = 15.f;
+constexpr int WEIGHT_SHIFT = 15;
+constexpr float WEIGHT_UNIT = 1.f / (1 << WEIGHT_SHIFT);
+constexpr int SCALES_NEAR = 64;      // exponents of values' scales this close take the short way to a denominator
 constexpr int NO_PAGE = -1000;       // in an exponent's place
 
 template <int HD>
@@ -100,6 +104,13 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// ... down to float32's subnormal numbers
+__device__ __forceinline__ float ex2_subnormal(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // Shared memory holds a split's block in lines of 128 bytes, 16-byte pieces swizzled: piece c of line l is at c ^ (l & 7).
 __device__ __forceinline__ int swizzled(int line, int piece) { return line * 128 + ((piece ^ (line & 7)) << 4); }
 
@@ -121,13 +132,13 @@ __device__ __forceinline__ int key_offset(int key, int piece) {
 template <int HD>
 __device__ __forceinline__ int value_offset(int group, int g, int i) { return swizzled(group * (HD / 32) + i, g); }
 
-// What outputs relative to the base-2 maximum `top` are multiplied by: one over the sum of the weights, of which the head's
-// sink (in natural units) is one more without a key.
+// What outputs relative to the base-2 maximum `top` are multiplied by, next to WEIGHT_UNIT: one over the sum of the weights,
+// of which the head's sink (in natural units) is one more without a key.
 __device__ __forceinline__ float finish(float top, float sum, const float* sinks, int head) {
   if (sinks == nullptr) return sum > 0.f || sum != sum ? 1.f / sum : 0.f;
   const float sink = sinks[head] * 1.4426950408889634f, m = fmaxf(top, sink);
-  const float f = top == -INFINITY ? 0.f : ex2(top - m);
-  return f / (sum * f + ex2(sink - m));
+  const float half = top == -INFINITY ? 0.f : ex2(0.5f * (top - m));
+  return half * half / (sum * half * half + ex2(sink - m));
 }
 
 // Two neighbouring outputs, turned by position * frequency of their pair where a table is given.
@@ -167,6 +178,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
   int* s_cum = s_pos + n_seqs;                                     // [n_seqs + 1] (request, split) pairs before it
   __shared__ __align__(8) uint64_t full[SLOTS], empty[SLOTS];
   __shared__ int s_exp[SLOTS][2][TILES];     // exponents of the keys' and the values' boxes, with the keys' slot
+  __shared__ int s_apart[SLOTS];             // whether the values' scales of a run so far are far apart, with the keys' slot
   __shared__ __align__(8) uint2 s_weights[TILES][32];  // the second product's right operand
   __shared__ __align__(8) float s_top[4][MAX_COLUMNS], s_sum[4][MAX_COLUMNS];
   __shared__ __align__(16) int s_run[2][8];  // the block's partials: request, slice, token, position (-1: none), blocks from and to
@@ -280,8 +292,9 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     // stale pages where a prompt's write is followed at once.)
     pdl_wait();
     int slot = 0, use = 0;
+    int run_low = KV8_HIGHEST, run_top = KV8_LOWEST;  // exponents of the values' scales in the run so far
     for (int i = 0; i < count; ++i) {
-      const int k0 = (w.first + w.split) * SPLIT, g = w.slice / n_sub;
+      const int k0 = (w.first + w.split) * SPLIT, g = w.slice / n_sub, seq = w.seq, slice = w.slice;
       const size_t block = (size_t)max(page, 0) * n_kv_heads + g;
       const uint32_t ks = page >= 0 ? ld_global_4(k_scales + block) : 0u, vs = page >= 0 ? ld_global_4(v_scales + block) : 0u;
       const unsigned valid = __ballot_sync(0xffffffffu, page >= 0);
@@ -307,10 +320,15 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
         advance(w);
         next_page = page_of(w);
       }
+      const int ev = page >= 0 ? exponent_of_scale(__uint_as_float(vs)) : 0;
       if (lane < n_boxes) {
         s_exp[k_slot][0][lane] = page >= 0 ? exponent_of_scale(__uint_as_float(ks)) : NO_PAGE;
-        s_exp[k_slot][1][lane] = page >= 0 ? exponent_of_scale(__uint_as_float(vs)) : 0;
+        s_exp[k_slot][1][lane] = ev;
       }
+      run_low = min(run_low, __reduce_min_sync(0xffffffffu, page >= 0 ? ev : KV8_HIGHEST));
+      run_top = max(run_top, __reduce_max_sync(0xffffffffu, page >= 0 ? ev : KV8_LOWEST));
+      if (lane == 0) s_apart[k_slot] = run_top - run_low > SCALES_NEAR;
+      if (w.seq != seq || w.slice != slice) run_low = KV8_HIGHEST, run_top = KV8_LOWEST;  // the next item begins a run
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&full[k_slot]);
@@ -401,6 +419,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
       mbar_wait(&full[slot], use & 1, status, &gave_up);
       float s[2][4];
       int ek[2], ev[2];
+      const bool apart = s_apart[slot] != 0;
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
         const int box = (warp * 32 + mt * 16) >> box_shift;
@@ -470,18 +489,22 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
         top[1] = fmaxf(top[1], other.y);
       }
       // what the run holds so far, relative to the new maximum
-      float keep[2];
+      float keep[2], down[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        keep[h] = run_top[h] == -INFINITY ? 0.f : ex2(run_top[h] - top[h]);
+        down[h] = run_top[h] == -INFINITY ? -INFINITY : run_top[h] - top[h];
+        keep[h] = ex2(down[h]);
         run_top[h] = top[h];
-        run_sum[h] *= keep[h];
       }
       const float base[2] = {WEIGHT_SHIFT - (top[0] == -INFINITY ? 0.f : top[0]), WEIGHT_SHIFT - (top[1] == -INFINITY ? 0.f : top[1])};
-      // The softmax's own weight is the value's weight over its scale, 2^-f: a multiplication where the scales are near
-      // one another.  (A weight that is zero in float32 is 2^-141 of the largest: over scales up to 2^50 apart 2^-41.)
-      if (max(abs(ev[0]), abs(ev[1])) <= 50) {
-        const float inv[2] = {exp2_int(-ev[0]), exp2_int(-ev[1])};
+      // The softmax's own weight is the value's weight over its scale, 2^-f: a multiplication where the scales of the run are
+      // near one another.  (A weight that is zero in float32 is 2^-141 of the largest, over scales 2^64 apart 2^-77 of the
+      // denominator; what `keep` loses of an earlier sum is 2^-62.)  Elsewhere an exponential of its own, to 2^-149 where
+      // the denominator is 2^-100 or more.
+      if (!apart) {
+        run_sum[0] *= keep[0];
+        run_sum[1] *= keep[1];
+        const float inv[2] = {exp2_int(-ev[0] - WEIGHT_SHIFT), exp2_int(-ev[1] - WEIGHT_SHIFT)};
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
@@ -491,12 +514,17 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
           }
       } else {
 #pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float half = ex2(0.5f * down[h]);
+          run_sum[h] = run_sum[h] * half * half;
+        }
+#pragma unroll
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float x = s[mt][e] + base[e & 1];
             s[mt][e] = ex2(x);
-            run_sum[e & 1] += ex2(x - fe[mt]);
+            run_sum[e & 1] += ex2_subnormal(x - (fe[mt] + WEIGHT_SHIFT));
           }
       }
       // the weights as the 8-column operand: an 8 x 8 transposition in registers for each half tile
@@ -585,7 +613,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int head = head0 + min(2 * t4 + e, heads - 1);
-          f[e] = finish(run_top[e] - WEIGHT_SHIFT, sum[e], sinks, head);
+          f[e] = finish(run_top[e], sum[e], sinks, head);
         }
 #pragma unroll
         for (int c = 0; c < MINE; ++c)
@@ -597,7 +625,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
               const int piece = HALVES == 2 ? warp + 4 * c : warp >> 1, which = HALVES == 2 ? h : warp & 1;
               const int d = 4 * (g8 + 8 * piece) + 2 * which;
               if (2 * t4 + e < heads)
-                store_pair(dst + (2 * t4 + e) * HD + d, o[c][h][e] * f[e], o[c][h][2 + e] * f[e], out_freqs, d / 2, at.p);
+                store_pair(dst + (2 * t4 + e) * HD + d, o[c][h][e] * WEIGHT_UNIT * f[e], o[c][h][2 + e] * WEIGHT_UNIT * f[e],
+                           out_freqs, d / 2, at.p);
             }
         continue;
       }
@@ -619,7 +648,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
 #pragma unroll
         for (int e = 0; e < 2; ++e)
           if (2 * t4 + e < heads)
-            *reinterpret_cast<float2*>(part + (2 * t4 + e) * run_stride<HD>() + HD) = make_float2(run_top[e] - WEIGHT_SHIFT, sum[e]);
+            *reinterpret_cast<float2*>(part + (2 * t4 + e) * run_stride<HD>() + HD) = make_float2(run_top[e], sum[e]);
       if (tid == 0) {
         *reinterpret_cast<int4*>(s_run[which_run]) = make_int4(at.seq, at.slice, tok, at.p);
         s_run[which_run][4] = block_of(run0);
@@ -672,21 +701,33 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
                          : "l"(from + d)
                          : "memory");
           }
-          float top = m;
+          float top = m, low = m == -INFINITY ? INFINITY : m;
 #pragma unroll
           for (int u = 0; u < FLIGHT; ++u) {
+            low = fminf(low, ml[u].x);
             if (b0 + u > last_block) ml[u] = make_float2(-INFINITY, 0.f);  // (the last one once more: nothing)
             top = fmaxf(top, ml[u].x);
           }
           const float keep = m == -INFINITY ? 0.f : ex2(m - top);
+          const bool apart = low - top < -SCALES_NEAR;
+          if (apart) {
+            const float half = m == -INFINITY ? 0.f : ex2(0.5f * (m - top));
+            l = l * half * half;
+#pragma unroll
+            for (int u = 0; u < FLIGHT; ++u) {
+              const float h = ml[u].x == -INFINITY ? 0.f : ex2(0.5f * (ml[u].x - top));
+              l += h * ml[u].y * h;
+            }
+          } else {
+            l *= keep;
+          }
           m = top;
-          l *= keep;
 #pragma unroll
           for (int e = 0; e < 4; ++e) a[e] *= keep;
 #pragma unroll
           for (int u = 0; u < FLIGHT; ++u) {
             const float f = ml[u].x == -INFINITY ? 0.f : ex2(ml[u].x - top);
-            l += f * ml[u].y;
+            if (!apart) l += f * ml[u].y;
             a[0] += f * v[u].x;
             a[1] += f * v[u].y;
             a[2] += f * v[u].z;
@@ -703,6 +744,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
           }
         }
         const float f = finish(m, l, sinks, head0 + r);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] *= WEIGHT_UNIT;
         store_pair(dst + r * HD + d, a[0] * f, a[1] * f, out_freqs, d / 2, p);
         store_pair(dst + r * HD + d + 2, a[2] * f, a[3] * f, out_freqs, d / 2 + 1, p);
       }
