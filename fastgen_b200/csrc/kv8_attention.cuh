@@ -454,8 +454,9 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           if constexpr (CAPPED) {
-            s[mt][h] = capped_score(s[mt][h] * ks * un[h], scale_log2, cap_log2, scale_by_cap) + fe[mt];
-            s[mt][2 + h] = capped_score(s[mt][2 + h] * ks * un[h], scale_log2, cap_log2, scale_by_cap) + fe[mt];
+            // (the query's power of two first: large keys' sums would leave float32 before a small query's brings them back)
+            s[mt][h] = capped_score(s[mt][h] * un[h] * ks, scale_log2, cap_log2, scale_by_cap) + fe[mt];
+            s[mt][2 + h] = capped_score(s[mt][2 + h] * un[h] * ks, scale_log2, cap_log2, scale_by_cap) + fe[mt];
           } else {
             const float f = ks * (un[h] * scale_log2);
             s[mt][h] = fmaf(s[mt][h], f, fe[mt]);

@@ -78,3 +78,19 @@ def test_values_far_apart(ops, scores, magnitudes, copies, sink, page):
     q = torch.zeros(1, size)
     q[0, 0] = 1.0
     _check_copies(ops, cache, q, n, 1, copies, 1.0, torch.tensor([2.0], device=DEV) if sink else None)
+
+
+@pytest.mark.parametrize("up", [-60, 0, 60, 108])
+def test_capped_scores_of_small_queries_and_large_keys(ops, up):
+    """Keys of 2^up against queries of 2^(-up - 4): the scores are ordinary ones, and capped as such."""
+    size, n = 128, 200
+    g = torch.Generator().manual_seed(3)
+    k = torch.rand(n, 1, generator=g).expand(n, size) * 1.7 * 2.0 ** up
+    v = torch.randn(n, size, generator=g)
+    cache = _copies(ops, k, v, 1, 64, 1)
+    q = torch.full((1, size), 1.99 * 2.0 ** (-up - 5), dtype=torch.bfloat16, device=DEV)
+    out = torch.empty_like(q)
+    ctx = _context([n - 1], [1])
+    ops.attention(q, out, cache.memory, ctx, 1, 1, size, None, 0.5, softcap=3.0)
+    ops.check_status()
+    _check(out, *_attention(cache, q, ctx, 1, 0.5, softcap=3.0))
