@@ -16,8 +16,8 @@ namespace fg_kv8 {
 // Bound by instructions at many tokens (each key/value head's block computes the angles anew) and by latencies at few: a block is a
 // chain of positions, pages, rows, angles and codes.  Steps of many tokens take stretches of 64 tokens (PER = 4), a page of
 // the usual size: with 16, three of four blocks found no run and left.  Queries have blocks of their own, a warp a token.
-// (32 / 8 heads of 128: 2,048 prompt tokens beside 20 single ones 14.2 us, the write in 16 bits 9.4; 8,192 tokens 65.7 and 43.7.
-// Before codes in doubt were settled in 64 bits: 12.3 and 53.8; with queries in the stretches' blocks and each thread looking
+// (32 / 8 heads of 128: 2,048 prompt tokens beside 20 single ones 14.4 us, the write in 16 bits 9.4; 8,192 tokens 66.4 and 43.7.
+// Without the exponents in doubt 14.1 and 65.6, without codes in doubt 12.3 and 53.8; with queries in the stretches' blocks and each thread looking
 // through all places for the runs: 19.2 and 67.2.)
 // ---------------------------------------------------------------------------------
 constexpr int WRITE_WARPS = 16, WRITE_THREADS = 32 * WRITE_WARPS;
@@ -69,6 +69,110 @@ __device__ __noinline__ float2 turned_exactly(const __nv_bfloat16* at, double w0
   return make_float2(narrowed((a * cs - b * sn) * magnitude), narrowed((b * cs + a * sn) * magnitude));
 }
 
+// A page's exponent: from the run's largest magnitude and, behind cached entries, no lower than theirs.
+__device__ __forceinline__ int run_exponent(float amax, int slot, float before, int& old_e) {
+  int e = scale_exponent(amax);
+  old_e = e;
+  if (slot > 0) {
+    old_e = exponent_of_scale(before);
+    e = max(e, old_e);
+  }
+  return e;
+}
+
+// Cached entries before `slot` rounded again at a larger scale, by `n` threads of which this is number `i`.
+template <int HD>
+__device__ __forceinline__ void rescale_entries(unsigned char* base, bool is_v, int slot, float f, int i, int n) {
+  const int whole = is_v ? (slot & ~3) * HD : slot * HD;  // bytes of whole rows (of whole groups of four rows)
+  for (int at = i * 4; at < whole; at += n * 4) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(base + at);
+    *w = rescaled(ld_global_4(w), f);
+  }
+  if (is_v && (slot & 3)) {
+    const uint32_t mask = (1u << (8 * (slot & 3))) - 1u;  // tokens of the last group that are cached
+    for (int d = i; d < HD; d += n) {
+      uint32_t* w = reinterpret_cast<uint32_t*>(base + whole) + d;
+      const uint32_t old = ld_global_4(w);
+      *w = (old & ~mask) | (rescaled(old, f) & mask);
+    }
+  }
+}
+
+// A lane's codes of one row.
+template <int HD>
+__device__ __forceinline__ void store_codes(unsigned char* base, bool is_v, const float (&x)[HD / 32], int slot, float inv, int lane) {
+  constexpr int E = HD / 32;
+  uint32_t c[E / 2];
+#pragma unroll
+  for (int i = 0; i < E / 2; ++i) c[i] = codes_of(x[2 * i] * inv, x[2 * i + 1] * inv);
+  if (!is_v) {
+    unsigned char* dst = base + slot * HD + lane * E;
+    if constexpr (E == 2) *reinterpret_cast<uint16_t*>(dst) = (uint16_t)c[0];
+    else if constexpr (E == 4) *reinterpret_cast<uint32_t*>(dst) = c[0] | (c[1] << 16);
+    else *reinterpret_cast<uint2*>(dst) = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+  } else {
+    unsigned char* dst = base + (slot >> 2) * (4 * HD) + lane * (4 * E) + (slot & 3);
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+      dst[8 * i] = (unsigned char)c[i];
+      dst[8 * i + 4] = (unsigned char)(c[i] >> 8);
+    }
+  }
+}
+
+// A run of `n` tokens from slot `slot` and position p0 on, its keys (or its values) all in 64 bits, by the whole block, or by one
+// warp without an s_amax: for runs whose largest magnitude float32 cannot tell from a border of the scales.  src: the run's first row; rstd: the norm's factor of
+// its first token or null, `rstd_stride` apart; norm_w its weights or null; big: pairs that `magnitude` multiplies.
+template <int HD>
+__device__ __noinline__ void exact_run(const __nv_bfloat16* src, int src_stride, bool is_v, int n, int slot, int p0, const float* freqs,
+                                       const float* rstd, int rstd_stride, const float* norm_w, float magnitude, int big,
+                                       unsigned char* base, float* scale, float* s_amax) {
+  constexpr int E = HD / 32;
+  const int lane = threadIdx.x & 31, warp = s_amax ? threadIdx.x >> 5 : 0, warps = s_amax ? WRITE_WARPS : 1;
+  auto sync = [&]() {
+    if (s_amax) __syncthreads();
+    else __syncwarp();
+  };
+  auto row = [&](float (&x)[E], int i) {
+#pragma unroll 1
+    for (int j = 0; j < E / 2; ++j) {
+      const int pair = lane * (E / 2) + j;
+      const __nv_bfloat16* at = src + (size_t)i * src_stride + 2 * pair;
+      double w0 = rstd ? rstd[(size_t)i * rstd_stride] : 1.f, w1 = w0;
+      if (norm_w) w0 *= norm_w[2 * pair], w1 *= norm_w[2 * pair + 1];
+      const float2 v = freqs || rstd ? turned_exactly(at, w0, w1, freqs ? (float)(p0 + i) * freqs[pair] : 0.f, freqs && pair < big ? magnitude : 1.f)
+                                     : make_float2(__bfloat162float(at[0]), __bfloat162float(at[1]));
+      x[2 * j] = fabsf(v.x) == INFINITY ? __int_as_float(0x7fffffff) : v.x;
+      x[2 * j + 1] = fabsf(v.y) == INFINITY ? __int_as_float(0x7fffffff) : v.y;
+    }
+  };
+  float x[E], amax = 0.f;
+  const float before = slot > 0 ? __uint_as_float(ld_global_4(scale)) : 1.f;
+#pragma unroll 1
+  for (int i = warp; i < n; i += warps) {
+    row(x, i);
+#pragma unroll
+    for (int j = 0; j < E; ++j) amax = fmaxf(amax, fabsf(x[j]));
+  }
+  amax = warp_max(amax);
+  if (s_amax) {
+    __syncthreads();
+    if (lane == 0) s_amax[warp] = amax;
+    __syncthreads();
+    amax = warp_max(s_amax[lane & (WRITE_WARPS - 1)]);
+  }
+  int old_e;
+  const int e = run_exponent(amax, slot, before, old_e);
+  if (e > old_e) rescale_entries<HD>(base, is_v, slot, exp2_int(max(old_e - e, -126)), warp * 32 + lane, warps * 32);
+  sync();  // rescaled entries share words with new ones; every thread has read the old scale
+#pragma unroll 1
+  for (int i = warp; i < n; i += warps) {
+    row(x, i);
+    store_codes<HD>(base, is_v, x, slot + i, exp2_int(-e), lane);
+  }
+  if (warp + lane == 0 && (slot == 0 || e > old_e)) *scale = exp2_int(e);
+}
+
 template <int HD, bool VEC, int PER>
 __global__ void __launch_bounds__(WRITE_THREADS, HD <= 128 ? 2 : 1)
 kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, const __nv_bfloat16* k, int k_stride,
@@ -81,6 +185,7 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
   constexpr int E = HD / 32, STRETCH = WRITE_WARPS * PER;
   __shared__ int s_len[STRETCH], s_page[STRETCH], s_pos[STRETCH];
   __shared__ float s_amax[2][WRITE_WARPS];
+  __shared__ int s_marked;
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   // blocks of keys and values first, the heads of a stretch side by side; then those of queries
@@ -209,6 +314,7 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
       s_pos[warp * PER + u] = p;
     }
   }
+  if (threadIdx.x == 0) s_marked = 0;
   any_long = __syncthreads_or(any_long);
   pdl_wait();
 
@@ -227,52 +333,11 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
     }
     return a;
   };
-  // the page's exponent: from the run's largest magnitude and, behind cached entries, no lower than theirs
-  auto exponents = [&](float amax, int slot, float before, int& old_e) {
-    int e = scale_exponent(amax);
-    old_e = e;
-    if (slot > 0) {
-      old_e = exponent_of_scale(before);
-      e = max(e, old_e);
-    }
-    return e;
-  };
-  // cached entries before `slot` rounded again at a larger scale, by `n` threads of which this is number `i`
   auto rescale = [&](int kv, size_t block, int slot, float f, int i, int n) {
-    unsigned char* base = pool[kv] + block * (size_t)page_size * HD;
-    const int whole = kv ? (slot & ~3) * HD : slot * HD;  // bytes of whole rows (of whole groups of four rows)
-    for (int at = i * 4; at < whole; at += n * 4) {
-      uint32_t* w = reinterpret_cast<uint32_t*>(base + at);
-      *w = rescaled(ld_global_4(w), f);
-    }
-    if (kv && (slot & 3)) {
-      const uint32_t mask = (1u << (8 * (slot & 3))) - 1u;  // tokens of the last group that are cached
-      for (int d = i; d < HD; d += n) {
-        uint32_t* w = reinterpret_cast<uint32_t*>(base + whole) + d;
-        const uint32_t old = ld_global_4(w);
-        *w = (old & ~mask) | (rescaled(old, f) & mask);
-      }
-    }
+    rescale_entries<HD>(pool[kv] + block * (size_t)page_size * HD, kv, slot, f, i, n);
   };
-  // a lane's codes of one row
   auto store_row = [&](int kv, const float (&x)[E], size_t block, int slot, float inv) {
-    unsigned char* base = pool[kv] + block * (size_t)page_size * HD;
-    uint32_t c[E / 2];
-#pragma unroll
-    for (int i = 0; i < E / 2; ++i) c[i] = codes_of(x[2 * i] * inv, x[2 * i + 1] * inv);
-    if (!kv) {
-      unsigned char* dst = base + slot * HD + lane * E;
-      if constexpr (E == 2) *reinterpret_cast<uint16_t*>(dst) = (uint16_t)c[0];
-      else if constexpr (E == 4) *reinterpret_cast<uint32_t*>(dst) = c[0] | (c[1] << 16);
-      else *reinterpret_cast<uint2*>(dst) = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
-    } else {
-      unsigned char* dst = base + (slot >> 2) * (4 * HD) + lane * (4 * E) + (slot & 3);
-#pragma unroll
-      for (int i = 0; i < E / 2; ++i) {
-        dst[8 * i] = (unsigned char)c[i];
-        dst[8 * i + 4] = (unsigned char)(c[i] >> 8);
-      }
-    }
+    store_codes<HD>(pool[kv] + block * (size_t)page_size * HD, kv, x, slot, inv, lane);
   };
   // Turned numbers are off by less than 2^-21 of their pair's magnitudes (sine and cosine 2^-23, two products and a sum 2^-24
   // each, and the square root of two from a pair to its turn), with a norm's factors or a magnitude less than 2^-20.  Where that
@@ -302,6 +367,21 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
       }
     }
   };
+  // The largest magnitude is off by less than 2^-19 of itself, for its pair's other number is no larger.  Where that leaves the
+  // exponent in doubt (the borders are 1.75 times powers of two: within 32 of its last places, 2^-23 each, of one),
+  // the run is marked by a negative length and left to exact_run, behind the others.  (Its keys or values may have been written
+  // before: once more is the same.)
+  auto in_doubt = [&](int kv, float amax) {
+    return __builtin_expect(turned[kv] && ((__float_as_uint(amax) - (0x600000u - 32u)) & 0x7fffffu) <= 64u, 0);
+  };
+  auto exact = [&](int kv, int t, int n, int p, int page, float* amax) {
+    const int slot = p & (page_size - 1);
+    const size_t block = (size_t)page * n_kv_heads + g;
+    const float* factor = kv || rstd == nullptr ? nullptr : rstd_heads ? rstd + (size_t)t * rstd_heads + n_heads + g : rstd + 2 * (size_t)t + 1;
+    exact_run<HD>(src[kv] + (size_t)t * src_stride[kv], src_stride[kv], kv, n, slot, p, kv ? v_freqs : freqs, factor,
+                  rstd_heads ? rstd_heads : 2, kv ? nullptr : norm_w, kv ? 1.f : magnitude, kv ? 0 : rot_pairs,
+                  pool[kv] + block * (size_t)page_size * HD, scales[kv] + block, amax);
+  };
   auto scale_before = [&](int kv, size_t block, int slot) {
     return slot > 0 ? __uint_as_float(ld_global_4(scales[kv] + block)) : 1.f;
   };
@@ -315,6 +395,7 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
     load_lane<E, VEC>(raw[0], src[0] + (size_t)t * src_stride[0], lane);
     load_lane<E, VEC>(raw[1], src[1] + (size_t)t * src_stride[1], lane);
     const float before[2] = {scale_before(0, block, slot), scale_before(1, block, slot)};
+    bool left = false;
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
       float x[E];
@@ -326,8 +407,12 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
         turn(x, sn, cs);
       }
       const float amax = warp_max(row_amax(x));
+      if (in_doubt(kv, amax)) {
+        left = true;
+        continue;
+      }
       int old_e;
-      const int e = exponents(amax, slot, before[kv], old_e);
+      const int e = run_exponent(amax, slot, before[kv], old_e);
       if (e > old_e) {
         rescale(kv, block, slot, exp2_int(max(old_e - e, -126)), lane, 32);
         __syncwarp();
@@ -336,8 +421,18 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
       store_row(kv, x, block, slot, exp2_int(-e));
       if (lane == 0 && (slot == 0 || e > old_e)) scales[kv][block] = exp2_int(e);
     }
+    if (left && lane == 0) s_len[warp * PER + u] = -1, s_marked = 1;
   }
-  if (!any_long) return;
+  if (!any_long) {
+    __syncwarp();
+#pragma unroll 1
+    for (int u = 0; u < PER; ++u)
+      if (__builtin_expect(s_len[warp * PER + u] < 0, 0)) {
+        exact(0, mine + u, 1, s_pos[warp * PER + u], s_page[warp * PER + u], nullptr);
+        exact(1, mine + u, 1, s_pos[warp * PER + u], s_page[warp * PER + u], nullptr);
+      }
+    return;
+  }
 
   unsigned todo = 0;  // runs of two and more tokens among 32 of the stretch's tokens
 #pragma unroll 1
@@ -408,9 +503,14 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
     __syncthreads();
     int e[2], old_e[2];
 #pragma unroll
+    for (int kv = 0; kv < 2; ++kv) amax[kv] = warp_max(s_amax[kv][lane & (WRITE_WARPS - 1)]);
+    if (__builtin_expect(in_doubt(0, amax[0]) || in_doubt(1, amax[1]), 0)) {  // (every thread has the same numbers)
+      if (threadIdx.x == 0) s_len[w] = -n, s_marked = 1;
+      continue;
+    }
+#pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
-      amax[kv] = warp_max(s_amax[kv][lane & (WRITE_WARPS - 1)]);
-      e[kv] = exponents(amax[kv], slot, before[kv], old_e[kv]);
+      e[kv] = run_exponent(amax[kv], slot, before[kv], old_e[kv]);
       if (e[kv] > old_e[kv]) rescale(kv, block, slot, exp2_int(max(old_e[kv] - e[kv], -126)), threadIdx.x, WRITE_THREADS);
     }
     if (slot > 0) __syncthreads();  // rescaled entries share words with new ones; every thread has read the old scales
@@ -454,6 +554,15 @@ kv8_write_kernel(const __nv_bfloat16* q, int q_stride, __nv_bfloat16* q_out, con
       const int mine = kv ? e[1] : e[0], old = kv ? old_e[1] : old_e[0];
       if (slot == 0 || mine > old) scales[kv][block] = exp2_int(mine);
     }
+  }
+
+  __syncthreads();
+  if (s_marked == 0) return;
+#pragma unroll 1
+  for (int w = 0; w < STRETCH; ++w) {
+    if (s_len[w] >= 0) continue;
+    exact(0, t0 + w, -s_len[w], s_pos[w], s_page[w], s_amax[0]);
+    exact(1, t0 + w, -s_len[w], s_pos[w], s_page[w], s_amax[1]);
   }
 }
 

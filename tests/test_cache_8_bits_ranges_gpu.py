@@ -7,7 +7,7 @@ Tolerances are those of the other tests of this cache: outputs of attention with
 import pytest
 import torch
 
-from test_cache_8_bits_gpu import DEV, Cache, _attention, _check, _context
+from test_cache_8_bits_gpu import DEV, Cache, _attention, _check, _context, _exponent
 
 pytestmark = pytest.mark.gpu
 
@@ -94,3 +94,74 @@ def test_capped_scores_of_small_queries_and_large_keys(ops, up):
     ops.attention(q, out, cache.memory, ctx, 1, 1, size, None, 0.5, softcap=3.0)
     ops.check_status()
     _check(out, *_attention(cache, q, ctx, 1, 0.5, softcap=3.0))
+
+
+def _near_borders(size, page, place, magnitude, pairs, seed, factors=None):
+    """Rotations (pair, position at slot ``place`` of a page, the two numbers) whose larger result lies within 2^-22 of
+    448 * 2^e, and that result in 64 bits."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    freqs = (10000.0 ** (-torch.arange(size // 2, device=DEV).double() * 2 / size)).float()
+    found = []
+    for _ in range(24):
+        n = 20_000_000
+        pair = torch.randint(1, size // 2, (n,), generator=g, device=DEV)
+        pos = (torch.randint(1, 4000 // page, (n,), generator=g, device=DEV) * page + place).to(torch.int32)
+        a, b = (torch.randn(n, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+        angle = (pos.float() * freqs[pair]).double()
+        c, s = torch.cos(angle), torch.sin(angle)
+        if magnitude != 1.0:
+            f = torch.where(pair < pairs, magnitude, 1.0).double()
+            c, s = c * f, s * f
+        x, y = a.double(), b.double()
+        rstd = torch.ones(n, device=DEV)
+        if factors is not None:
+            rstd = 0.5 + torch.rand(n, generator=g, device=DEV)
+            x, y = x * rstd.double() * factors.double()[2 * pair], y * rstd.double() * factors.double()[2 * pair + 1]
+        big = torch.maximum((x * c - y * s).abs(), (y * c + x * s).abs())
+        m, _e = torch.frexp(big)
+        hit = torch.nonzero((m - 0.875).abs() < 0.875 * 2.0 ** -22).flatten()
+        found.append((pair[hit], pos[hit], a[hit], b[hit], rstd[hit], big[hit]))
+    return freqs, [torch.cat(x) for x in zip(*found)]
+
+
+@pytest.mark.parametrize("size,page", [(64, 16), (128, 64), (256, 256)])
+@pytest.mark.parametrize("way", ["single", "behind", "run", "run behind"])
+@pytest.mark.parametrize("option", ["keys", "values", "norm", "magnitude"])
+def test_scales_next_to_a_border(ops, size, page, way, option):
+    """A page whose largest turned number lies within 2^-22 of 448 * 2^e, on either side of it: the smallest 2^e at which 448
+    reaches that number's 64-bit value.  (Float32 sees one in ten of them on the wrong side.)"""
+    from dataclasses import replace
+    place = 0 if way == "single" else 3
+    first = 2 if "behind" in way else 0  # tokens of the page that are cached before
+    magnitude, pairs = (1.25, size // 4) if option == "magnitude" else (1.0, 0)
+    g = torch.Generator().manual_seed(size)
+    weights = (0.5 + torch.rand(size, generator=g)).to(DEV) if option == "norm" else None
+    freqs, (pair, pos, a, b, rstd, big) = _near_borders(size, page, place, magnitude, pairs, size + len(way), weights)
+    n = pair.numel()
+    assert n > 100
+    cache = Cache(ops, n, 1, 1, page, size)
+    table = cache.table.expand(-1, 4000 // page + 1).contiguous()
+    memory = replace(cache.memory, block_table=table)
+    tokens = 1 if way in ("single", "behind") else page // 2 + 7
+    begin = place if tokens == 1 else first
+    rows = torch.zeros(n, tokens, size, dtype=torch.bfloat16, device=DEV)
+    each = torch.arange(n, device=DEV)
+    rows[each, place - begin, 2 * pair] = a
+    rows[each, place - begin, 2 * pair + 1] = b
+    rows = rows.view(n * tokens, size)
+    nothing = torch.zeros_like(rows)
+    start = (pos // page * page)[:, None]
+    if first or tokens == 1 and place:
+        t = torch.arange(begin, device=DEV, dtype=torch.int32)
+        zeros = torch.zeros(n * begin, size, dtype=torch.bfloat16, device=DEV)
+        ops.rope_kv8_write(zeros, zeros, zeros, (start + t).flatten().to(torch.int32), each.repeat_interleave(begin).to(torch.int32),
+                           None, memory, 1, 1, size)
+    at = (start + begin + torch.arange(tokens, device=DEV)).flatten().to(torch.int32)
+    req = each.repeat_interleave(tokens).to(torch.int32)
+    norm = (rstd.repeat_interleave(tokens)[:, None].expand(-1, 2).contiguous(), weights, weights) if option == "norm" else None
+    k, v = (nothing, rows) if option == "values" else (rows, nothing)
+    ops.rope_kv8_write(nothing, k, v, at, req, freqs, memory, 1, 1, size, v_freqs=freqs if option == "values" else None, qk_norm=norm,
+                       magnitude=magnitude, rot_pairs=pairs)
+    ops.check_status()
+    scales = (memory.v_scales if option == "values" else memory.k_scales)[table[:, 0].long(), 0].double()
+    assert torch.equal(scales, torch.exp2(_exponent(big).double()))
