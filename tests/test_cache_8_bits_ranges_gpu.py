@@ -7,7 +7,7 @@ Tolerances are those of the other tests of this cache: outputs of attention with
 import pytest
 import torch
 
-from test_cache_8_bits_gpu import DEV, Cache, _attention, _check, _context, _exponent
+from test_cache_8_bits_gpu import DEV, Cache, _attention, _check, _context, _exponent, _nearest, _turned
 
 pytestmark = pytest.mark.gpu
 
@@ -165,3 +165,57 @@ def test_scales_next_to_a_border(ops, size, page, way, option):
     ops.check_status()
     scales = (memory.v_scales if option == "values" else memory.k_scales)[table[:, 0].long(), 0].double()
     assert torch.equal(scales, torch.exp2(_exponent(big).double()))
+
+
+@pytest.mark.parametrize("size,page,heads,kv", [(64, 16, 6, 2), (128, 64, 8, 4), (256, 128, 4, 2)])
+@pytest.mark.parametrize("option", ["plain", "values turned", "norm a token", "norm a head", "magnitude"])
+@pytest.mark.parametrize("wide", [0, 3])
+def test_all_codes_and_scales_of_mixed_steps(ops, size, page, heads, kv, option, wide):
+    """Portions and single tokens, from the start of a page, inside one and behind cached tokens, with rows on and off 16 bytes: every
+    code and every scale is the 64-bit numbers'.  (A million numbers: float32 leaves some 25 codes in doubt.)"""
+    g = torch.Generator().manual_seed(size + len(option) + wide)
+    tokens = 600_000 // (kv * size)
+    cached = [0, 5, page - 2, 2 * page + 1, page, 0, 3] + [page + i for i in range(20)]
+    new = [tokens // 2, tokens // 4, tokens // 4, 3 * page, 2, 1, 1] + [1] * 20
+    cache = Cache(ops, len(new), -(-(max(new) + 4 * page) // page), kv, page, size)
+    for s, c in enumerate(cached):
+        if c:
+            cache.fill(s, c, s, spread=2.0 ** (s % 3 - 1))
+    pos = torch.cat([torch.arange(c, c + n) for c, n in zip(cached, new)]).to(torch.int32).to(DEV)
+    req = torch.cat([torch.full((n,), s) for s, n in enumerate(new)]).to(torch.int32).to(DEV)
+    t = pos.numel()
+    q, k, v = (torch.randn(t, n * size + wide, generator=g).to(torch.bfloat16).to(DEV)[:, wide:] for n in (heads, kv, kv))
+    freqs = (10000.0 ** (-torch.arange(size // 2).double() * 2 / size)).float().to(DEV)
+    v_freqs = freqs.flip(0).contiguous() if option == "values turned" else None
+    magnitude, pairs = (1.25, size // 4) if option == "magnitude" else (1.0, 0)
+    k64, v64 = (x.double().reshape(t, kv, size) for x in (k, v))
+    norm = None
+    if option.startswith("norm"):
+        columns = 2 if option == "norm a token" else heads + kv
+        norm = ((0.5 + torch.rand(t, columns, generator=g)).to(DEV), torch.ones(heads * size, device=DEV), (0.5 + torch.rand(kv * size, generator=g)).to(DEV))
+        k64 = k64 * (norm[0][:, 1:2] if columns == 2 else norm[0][:, heads:]).double()[:, :, None] * norm[2].double().view(kv, size)
+    k64 = _turned(k64, pos, freqs, magnitude, pairs)
+    if v_freqs is not None:
+        v64 = _turned(v64, pos, v_freqs)
+    held = [cache.entries(s, max(c, 1)) for s, c in enumerate(cached)]
+    before = [cache.memory.k_scales.clone(), cache.memory.v_scales.clone()]
+    ops.rope_kv8_write(q, k, v, pos, req, freqs, cache.memory, heads, kv, size, v_freqs=v_freqs, qk_norm=norm, magnitude=magnitude, rot_pairs=pairs)
+    ops.check_status()
+    start = 0
+    for s, (c, n) in enumerate(zip(cached, new)):
+        got = cache.entries(s, c + n)
+        for which, mine in enumerate((k64, v64)):
+            scales = (cache.memory.k_scales, cache.memory.v_scales)[which]
+            for lp in range(c // page, (c + n - 1) // page + 1):
+                pid = int(cache.table[s, lp])
+                a, b = max(c, lp * page), min(c + n, (lp + 1) * page)
+                rows = mine[start + a - c : start + b - c].transpose(0, 1)
+                e = _exponent(rows.abs().amax((1, 2)))
+                if a > lp * page:
+                    e = torch.maximum(e, _exponent(before[which][pid].double() * 448))
+                unit = torch.exp2(e.double())
+                assert torch.equal(scales[pid].double(), unit), (s, lp, which)
+                unit = unit[:, None, None]
+                want = torch.cat([_nearest(held[s][which][:, lp * page : a] / unit), _nearest(rows / unit)], 1) * unit
+                assert torch.equal(got[which][:, lp * page : b], want), (s, lp, which)
+        start += n
