@@ -139,6 +139,9 @@ class LayerMemory:
     #: codes, keys as [n_pages, Hkv, page, hd], values as [n_pages, Hkv, page / 4, hd, 4] (four tokens' codes side by side)
     k_scales: Optional[torch.Tensor] = None
     v_scales: Optional[torch.Tensor] = None
+    #: ... and the pages in the compute type that its prompt portions are read from, one pool for all layers of a shape (keys,
+    #: values, tensor maps; see ``Ops.kv8_expanded``)
+    expanded: Optional[tuple] = None
 
 
 class StepMemories(list):

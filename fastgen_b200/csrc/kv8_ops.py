@@ -65,8 +65,8 @@ class Kv8Ops:
     """See the module; mixed into :class:`~fastgen_b200.csrc.ops.Ops`."""
 
     def _init_kv8(self) -> None:
-        # (pages, kv heads, page, head size) of an 8-bit cache -> its pages in bfloat16 as prompt portions read
-        # them (keys, values, tensor maps); every layer and group of these sizes fills the same pool in turn
+        # (pages, kv heads, page, head size) of caches in 8 bits without a pool of their own -> their pages in bfloat16 (see
+        # kv8_expanded)
         self._expanded = {}
         # head size -> partials and counters of the single-token attention over a cache in 8 bits
         self._kv8_buffers = {}
@@ -183,18 +183,29 @@ class Kv8Ops:
             pages.data_ptr(), n, k.data_ptr(), v.data_ptr(), page, n_pages, n_kv_heads, head_dim, self.status.data_ptr(), _ops._stream()))
         return k, v
 
+    def make_kv8_expanded(self, shape):
+        """Pages in bfloat16 for a cache in 8 bits of ``shape`` (pages, kv heads, page, head size): keys, values and their
+        tensor maps.  Prompt portions read such pages; all layers of a shape fill the same ones in turn."""
+        k = torch.zeros(shape, dtype=torch.bfloat16, device=self.device)
+        v = torch.zeros_like(k)
+        return k, v, self.make_kv_tensor_maps(k[None], v[None], shape[2])
+
     def kv8_expanded(self, memory):
-        """The pool that prompt portions over a cache of this shape read: keys and values in bfloat16 and their tensor
-        maps.  Made at the first call (not inside a graph capture) and kept."""
+        """What :meth:`make_kv8_expanded` made for ``memory``'s cache: the pool in ``memory.expanded``, as an engine's memories
+        have it.  For a memory without one, a pool for each shape, made at the first call (not inside a graph capture) and kept as
+        long as this object."""
         self._one_stream()
-        key = tuple(memory.k_pages.shape)
-        got = self._expanded.get(key)
+        shape = tuple(memory.k_pages.shape)
+        if memory.expanded is not None:
+            if tuple(memory.expanded[0].shape) != shape or memory.expanded[0].device != memory.k_pages.device:
+                raise ValueError(f"a cache in 8 bits of {shape} on {memory.k_pages.device} comes with the expanded pages of "
+                                 f"{tuple(memory.expanded[0].shape)} on {memory.expanded[0].device}")
+            return memory.expanded
+        got = self._expanded.get(shape)
         if got is None:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("the first prompt portion over a cache in 8 bits cannot be inside a graph capture")
-            k = torch.zeros(key, dtype=torch.bfloat16, device=memory.k_pages.device)
-            v = torch.zeros_like(k)
-            got = self._expanded[key] = (k, v, self.make_kv_tensor_maps(k[None], v[None], key[2]))
+            got = self._expanded[shape] = self.make_kv8_expanded(shape)
         return got
 
     def _one_stream(self) -> None:

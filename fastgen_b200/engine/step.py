@@ -232,9 +232,14 @@ class Engine:
         )
         self.memories = self.cache.memories()
         if cache_bits == 8:
+            # the pools that prompt portions read, one for each shape: this engine's own, as its cache is
+            expanded = {}
             for mem in self.memories:
                 if mem.k_scales is not None:
-                    self.ops.kv8_expanded(mem)  # the pool that prompt portions read: now, not in the middle of a step
+                    shape = tuple(mem.k_pages.shape)
+                    if shape not in expanded:
+                        expanded[shape] = self.ops.make_kv8_expanded(shape)
+                    mem.expanded = expanded[shape]
         self.last_h2d_bytes = 0
         if use_graphs is None:
             use_graphs = not bool(os.environ.get("FG_NO_CUDA_GRAPHS"))
