@@ -6,7 +6,7 @@ one power of two for each page and head (float32 ``[pages, kv heads]``); an entr
 
 from __future__ import annotations
 
-import dataclasses
+import threading
 from ctypes import c_float, c_int, c_void_p
 from typing import Optional
 
@@ -29,6 +29,7 @@ SIGNATURES = {
     "fg_kv8_decode_counters": [_I, _I, _I],
 }
 _libraries = {}
+_capturing = torch.cuda.is_current_stream_capturing
 
 
 def kv8(head_dim: int):
@@ -65,13 +66,14 @@ class Kv8Ops:
     """See the module; mixed into :class:`~fastgen_b200.csrc.ops.Ops`."""
 
     def _init_kv8(self) -> None:
-        # (pages, kv heads, page, head size) of caches in 8 bits without a pool of their own -> their pages in bfloat16 (see
-        # kv8_expanded)
+        # ((pages, kv heads, page, head size), stream) -> pages in bfloat16 of caches in 8 bits that have none of their own; the
+        # stream of captured calls is None (see kv8_expanded)
         self._expanded = {}
-        # head size -> partials and counters of the single-token attention over a cache in 8 bits
+        self._expanding = threading.Lock()  # from the filling of such a pool to the launch that reads it
+        # (head size, stream) -> partials and counters of the single-token attention over a cache in 8 bits; the stream of
+        # captured calls is None
         self._kv8_buffers = {}
         self._kv8_retired = []
-        self._kv8_stream = None  # whose work the two are used by
 
     def _clear_kv8(self) -> None:
         for counters in [*self._kv8_retired, *(count for _scratch, count in self._kv8_buffers.values())]:
@@ -190,51 +192,52 @@ class Kv8Ops:
         v = torch.zeros_like(k)
         return k, v, self.make_kv_tensor_maps(k[None], v[None], shape[2])
 
-    def kv8_expanded(self, memory):
+    def kv8_expanded(self, memory, stream: Optional[int] = None):
         """What :meth:`make_kv8_expanded` made for ``memory``'s cache: the pool in ``memory.expanded``, as an engine's memories
-        have it.  For a memory without one, a pool for each shape, made at the first call (not inside a graph capture) and kept as
-        long as this object."""
-        self._one_stream()
+        have it, which belongs to the cache's one stream.  For a memory without one, a pool for each shape and stream, made at the
+        first call (not inside a graph capture; captured calls take the first stream's) and kept as long as this object."""
         shape = tuple(memory.k_pages.shape)
         if memory.expanded is not None:
             if tuple(memory.expanded[0].shape) != shape or memory.expanded[0].device != memory.k_pages.device:
                 raise ValueError(f"a cache in 8 bits of {shape} on {memory.k_pages.device} comes with the expanded pages of "
                                  f"{tuple(memory.expanded[0].shape)} on {memory.expanded[0].device}")
             return memory.expanded
-        got = self._expanded.get(shape)
-        if got is None:
-            if torch.cuda.is_current_stream_capturing():
+        if _capturing():
+            got = self._expanded.get((shape, None))
+            if got is None:
                 raise RuntimeError("the first prompt portion over a cache in 8 bits cannot be inside a graph capture")
-            got = self._expanded[shape] = self.make_kv8_expanded(shape)
+            return got
+        key = shape, _ops._stream() if stream is None else stream
+        got = self._expanded.get(key)
+        if got is None:
+            got = self._expanded[key] = self.make_kv8_expanded(shape)
+            self._expanded.setdefault((shape, None), got)
         return got
 
-    def _one_stream(self) -> None:
-        """The work buffers of the cache in 8 bits belong to one stream at a time: a call on another stream than the last
-        one's is ordered behind what that one holds so far.  (Captured graphs of one :class:`Ops` are replayed one after
-        the other, as an engine does.)"""
-        stream = _ops._stream()
-        if stream == self._kv8_stream:
-            return
-        if not torch.cuda.is_current_stream_capturing():
-            if self._kv8_stream is not None:
-                torch.cuda.current_stream(self.device).wait_stream(torch.cuda.ExternalStream(self._kv8_stream, self.device))
-            self._kv8_stream = stream
-
-    def _kv8_work(self, lib, head_dim: int, counters: int):
-        """Scratch and zeroed counters of the single-token attention over a cache in 8 bits.  They grow outside graph captures
-        only; buffers that were outgrown stay alive, since captured graphs may hold their addresses."""
-        self._one_stream()
-        scratch, count = self._kv8_buffers.get(head_dim, (None, None))
-        if scratch is None or count.numel() < counters:
-            if torch.cuda.is_current_stream_capturing():
+    def _kv8_work(self, lib, head_dim: int, counters: int, stream: int):
+        """Scratch and zeroed counters of the single-token attention over a cache in 8 bits: of the stream, or of all
+        captured graphs, which are replayed one after the other.  They grow outside graph captures only; the graphs' ones that were
+        outgrown stay alive, since graphs hold their addresses."""
+        if _capturing():
+            got = self._kv8_buffers.get((head_dim, None))
+            if got is None or got[1].numel() < counters:
                 raise RuntimeError("the first single-token attention of a size over a cache in 8 bits cannot be inside a graph capture")
-            if scratch is None:
-                scratch = torch.empty(lib.fg_kv8_decode_scratch_floats(), dtype=torch.float32, device=self.device)
-            else:
-                self._kv8_retired.append(count)
-            count = torch.zeros(max(1024, 1 << (counters - 1).bit_length()), dtype=torch.int32, device=self.device)
-            self._kv8_buffers[head_dim] = (scratch, count)
-        return scratch, count
+            return got
+        got = self._kv8_buffers.get((head_dim, stream))
+        if got is None or got[1].numel() < counters:
+            n = max(1024, 1 << (counters - 1).bit_length())
+            for key in ((head_dim, stream), (head_dim, None)):
+                old = self._kv8_buffers.get(key)
+                if old is not None and old[1].numel() >= n:
+                    continue
+                scratch = old[0] if old is not None else torch.empty(lib.fg_kv8_decode_scratch_floats(), dtype=torch.float32,
+                                                                     device=self.device)
+                if old is not None:
+                    self._kv8_retired.append(old[1])
+                self._kv8_buffers[key] = (scratch, torch.zeros(n, dtype=torch.int32, device=self.device))
+            torch.cuda.current_stream(self.device).synchronize()  # graphs are replayed on any stream
+            got = self._kv8_buffers[head_dim, stream]
+        return got
 
     def _attention_kv8(self, q, out, memory, ctx, n_heads, n_kv_heads, head_dim, window, scale, out_freqs, keep_first,
                        softcap, sinks, chunk) -> bool:
@@ -248,31 +251,31 @@ class Kv8Ops:
         lib = kv8(head_dim)
         signed_window = -int(chunk) if chunk else int(window or 0)
         n_pages, page = memory.k_pages.shape[0], memory.page_size
-        singles = ctx.single_tokens()
+        singles, stream = ctx.single_tokens(), _ops._stream()
         longest = getattr(ctx, "longest", None)
         prompts = longest != 1 and ctx.attention_tiles(_ops.attention_tiling(n_heads, n_kv_heads, _ops.PREFILL_TMA_ROWS), 2).n > 0
         if prompts:
-            k, v, maps = self.kv8_expanded(memory)
-            _ops._check(lib, lib.fg_kv8_expand(
-                _ops._ptr(memory.k_pages), _ops._ptr(memory.v_pages), _ops._ptr(memory.k_scales), _ops._ptr(memory.v_scales), _ops._ptr(table),
-                table.shape[1], _ops._ptr(ctx.seq_slot), _ops._ptr(ctx.seq_start), _ops._ptr(ctx.seq_cached), ctx.n_seqs, _ops._ptr(k), _ops._ptr(v), page,
-                n_pages, n_kv_heads, head_dim, signed_window, _ops._ptr(self.status), _ops._stream()))
-            expanded = dataclasses.replace(memory, k_pages=k, v_pages=v, k_scales=None, v_scales=None, tensor_maps=maps,
-                                           layer_index=0)
-            self.attention(q, out, expanded, _PromptsOnly(ctx), n_heads, n_kv_heads, head_dim, window, scale,
-                           softcap=softcap, sinks=sinks, chunk=chunk)
+            with self._expanding:
+                k, v, maps = self.kv8_expanded(memory, stream)
+                _ops._check(lib, lib.fg_kv8_expand(
+                    _ops._ptr(memory.k_pages), _ops._ptr(memory.v_pages), _ops._ptr(memory.k_scales), _ops._ptr(memory.v_scales), _ops._ptr(table),
+                    table.shape[1], _ops._ptr(ctx.seq_slot), _ops._ptr(ctx.seq_start), _ops._ptr(ctx.seq_cached), ctx.n_seqs, _ops._ptr(k), _ops._ptr(v), page,
+                    n_pages, n_kv_heads, head_dim, signed_window, _ops._ptr(self.status), stream))
+                expanded = type(memory)(k_pages=k, v_pages=v, block_table=table, page_size=page, tensor_maps=maps)
+                self.attention(q, out, expanded, _PromptsOnly(ctx), n_heads, n_kv_heads, head_dim, window, scale,
+                               softcap=softcap, sinks=sinks, chunk=chunk)
         fused = out_freqs is not None and not prompts and singles.n > 0
         if singles.n:
             # a counter for every sequence and slice of up to eight heads of a group
             slices = n_kv_heads * -(-n_heads // n_kv_heads // 8)
-            scratch, counters = self._kv8_work(lib, head_dim, singles.n * slices)
+            scratch, counters = self._kv8_work(lib, head_dim, singles.n * slices, stream)
             maps = memory.tensor_maps
             _ops._check(lib, lib.fg_kv8_attention_decode(
                 q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), maps[0].ptr, maps[1].ptr, memory.layer_index,
                 memory.k_scales.data_ptr(), memory.v_scales.data_ptr(), table.data_ptr(), table.shape[1], page, n_pages,
                 ctx.pos.data_ptr(), singles.req.data_ptr(), singles.tok.data_ptr(), singles.n, n_heads, n_kv_heads, head_dim,
                 signed_window, float(scale), float(softcap or 0.0), scratch.data_ptr(), scratch.numel(), counters.data_ptr(),
-                counters.numel(), _ops._ptr(out_freqs) if fused else None, _ops._ptr(sinks), self.status.data_ptr(), _ops._stream()))
+                counters.numel(), _ops._ptr(out_freqs) if fused else None, _ops._ptr(sinks), self.status.data_ptr(), stream))
         return fused
 
 
