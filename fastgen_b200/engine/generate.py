@@ -151,7 +151,7 @@ class Fastgen:
         per_token = model.cache_bytes_per_token(1 if args.cache_bits == 8 else act_bytes)
         widest = max((getattr(l.ffn.params, "ffn_dim", model.args.dim) if l.ffn is not None else model.args.dim
                       for l in model.args.layers))
-        mp = mem_params(model.weight_bytes(), per_token, model.args.dim, widest, act_bytes,
+        mp = mem_params(model.weight_bytes() + model.expanded_weight_bytes(), per_token, model.args.dim, widest, act_bytes,
                         max(args.prefill_gb, 0.1), args.gpu_gb)
         mp.round_to(block)
         max_seq = args.max_seq

@@ -144,6 +144,20 @@ class Model:
             total += sum(2 * heads * size * 2 for heads, size, _page in shapes)
         return total
 
+    def _weights4(self) -> List[Weight4]:
+        """The matrices that are held in 4 bits."""
+        def of(part):
+            for v in vars(part).values():
+                if isinstance(v, Weight4):
+                    yield v
+                elif isinstance(v, Part):
+                    yield from of(v)
+        return [w for block in self.blocks for part in block.parts() for w in of(part)]
+
+    def expanded_weight_bytes(self) -> int:
+        """Bytes of the largest 16-bit copy of 4-bit weights: products of many tokens make one and give it back."""
+        return max((2 * w.numel() for w in self._weights4()), default=0)
+
     def weight_bytes(self) -> int:
         """Bytes of every tensor a step reads (fused buffers, embedding once if tied)."""
         seen, total = set(), 0

@@ -1,0 +1,29 @@
+"""What serving in fewer bits counts of its memory and its traffic."""
+
+import pytest
+import torch
+
+import helpers as H
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def _folder(tmp_path):
+    from fastgen_b200.weights import write_random_model
+    return write_random_model(tmp_path / "m", dict(H.TINY_D, intermediate_size=384), 3, dtype=torch.bfloat16, norm_jitter=0.1)
+
+
+def test_the_budget_holds_a_16_bit_copy_of_4_bit_weights(tmp_path):
+    """Steps of many tokens expand a matrix at a time: the cache gets what is left beside the largest."""
+    from fastgen_b200.engine import Fastgen, GenArgs, HfLoader
+    args = GenArgs(use_sampling=False, max_gen=4, cache_block=32, max_batch=2, gpu_gb=0.103, prefill_gb=0.1, weight_bits=4)
+    fg = Fastgen.build(HfLoader(_folder(tmp_path)), args, device=DEV)
+    cfg = H.TINY_D
+    rows = max(2 * 384, (cfg["num_attention_heads"] + 2 * cfg["num_key_value_heads"]) * cfg.get("head_dim", cfg["hidden_size"] // cfg["num_attention_heads"]))
+    largest = 2 * rows * cfg["hidden_size"]
+    assert fg.model.expanded_weight_bytes() == largest > 0
+    per_token = fg.model.cache_bytes_per_token(2)
+    expect = (int(0.103e9) - fg.model.weight_bytes() - largest - int(0.1e9)) // per_token
+    assert fg.max_seq == -(-expect // 32) * 32 and expect > 32
+    fg.destroy()
