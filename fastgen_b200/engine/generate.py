@@ -148,7 +148,7 @@ class Fastgen:
         self._log_cuda_mem()
 
         # pages: from max_seq, or from the memory budget (generate.py:206-236)
-        per_token = model.cache_bytes_per_token(1 if args.cache_bits == 8 else act_bytes)
+        per_token = model.cache_bytes_per_token(1 if args.cache_bits == 8 else act_bytes, block)
         widest = max((getattr(l.ffn.params, "ffn_dim", model.args.dim) if l.ffn is not None else model.args.dim
                       for l in model.args.layers))
         mp = mem_params(model.weight_bytes() + model.expanded_weight_bytes(), per_token, model.args.dim, widest, act_bytes,

@@ -9,6 +9,7 @@ the schedule; nothing in this file knows what a mixer or feed-forward does.
 
 from __future__ import annotations
 
+import math
 from typing import Dict, List, Optional, Sequence
 
 import torch
@@ -131,16 +132,21 @@ class Model:
     def kv_from(self) -> List[Optional[int]]:
         return [e.kv_from for e in self.args.schedule]
 
-    def cache_bytes_per_token(self, elt_size: int) -> int:
+    def cache_bytes_per_token(self, elt_size: int, page_size: Optional[int] = None) -> int:
         """Bytes of keys and values one token adds over all runs that own a cache.  An element of one byte is a cache in 8
-        bits: prompt portions read such pages from a pool of one layer in the compute type, which is counted too."""
+        bits: prompt portions read such pages from a pool of one layer in the compute type, which is counted too, as are, with the
+        engine's ``page_size``, the scales of a page's heads."""
         total = 0
+        scales = 0.0
         shapes = set()
         for spec, src in zip(self.cache_specs(), self.kv_from()):
             if spec is not None and src is None:
                 total += spec.n_pools * spec.n_kv_heads * spec.head_dim * elt_size
                 shapes.add((spec.n_kv_heads, spec.head_dim, spec.page_size))
+                page = spec.page_size or page_size
+                scales += 4 * spec.n_pools * spec.n_kv_heads / page if page else 0.0
         if elt_size == 1:
+            total += math.ceil(scales)
             total += sum(2 * heads * size * 2 for heads, size, _page in shapes)
         return total
 

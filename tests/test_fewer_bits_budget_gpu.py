@@ -27,3 +27,18 @@ def test_the_budget_holds_a_16_bit_copy_of_4_bit_weights(tmp_path):
     expect = (int(0.103e9) - fg.model.weight_bytes() - largest - int(0.1e9)) // per_token
     assert fg.max_seq == -(-expect // 32) * 32 and expect > 32
     fg.destroy()
+
+
+@pytest.mark.parametrize("page", [16, 64])
+def test_the_budget_holds_the_scales_of_an_8_bit_cache(tmp_path, page):
+    """What the pools of an engine hold for each token: codes, scales and the one layer that portions read."""
+    from fastgen_b200.engine import Fastgen, GenArgs, HfLoader
+    args = GenArgs(use_sampling=False, max_gen=4, cache_block=page, max_batch=2, gpu_gb=0.103, prefill_gb=0.1, cache_bits=8, num_cuda_graphs=1)
+    fg = Fastgen.build(HfLoader(_folder(tmp_path)), args, device=DEV)
+    grp = fg.engine.cache.groups[0]
+    held = {t.data_ptr(): t.numel() * t.element_size() for t in (grp.k_pages, grp.v_pages, grp.k_scales, grp.v_scales, *fg.engine.memories[0].expanded[:2])}
+    per_token = fg.model.cache_bytes_per_token(1, page)
+    assert sum(held.values()) / fg.max_seq <= per_token < sum(held.values()) / fg.max_seq + 1
+    expect = (int(0.103e9) - fg.model.weight_bytes() - int(0.1e9)) // per_token
+    assert fg.max_seq == -(-expect // page) * page and expect > page
+    fg.destroy()
