@@ -132,10 +132,11 @@ class Model:
     def kv_from(self) -> List[Optional[int]]:
         return [e.kv_from for e in self.args.schedule]
 
-    def cache_bytes_per_token(self, elt_size: int, page_size: Optional[int] = None) -> int:
+    def cache_bytes_per_token(self, elt_size: int, page_size: Optional[int] = None, expanded: bool = True) -> int:
         """Bytes of keys and values one token adds over all runs that own a cache.  An element of one byte is a cache in 8
-        bits: prompt portions read such pages from a pool of one layer in the compute type, which is counted too, as are, with the
-        engine's ``page_size``, the scales of a page's heads."""
+        bits: prompt portions read such pages from a pool of one layer in the compute type, which is counted too (steps of single
+        tokens do not touch it: ``expanded=False`` leaves it out), as are, with the engine's ``page_size``, the scales of a
+        page's heads."""
         total = 0
         scales = 0.0
         shapes = set()
@@ -147,6 +148,7 @@ class Model:
                 scales += 4 * spec.n_pools * spec.n_kv_heads / page if page else 0.0
         if elt_size == 1:
             total += math.ceil(scales)
+        if elt_size == 1 and expanded:
             total += sum(2 * heads * size * 2 for heads, size, _page in shapes)
         return total
 

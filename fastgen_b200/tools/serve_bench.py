@@ -193,8 +193,9 @@ def main() -> int:
     first_seconds, _, _ = run(reqs)
     steps0, pre0, log0 = fg.steps, fg.scheduler.n_preemptions, len(fg.step_log)
     seconds, n_out, errors = run(reqs)
-    roofline = roofline_of(fg.step_log[log0:], cfg, model.weight_bytes(), model.cache_bytes_per_token(args.cache_bits // 8),
-                           gen_args.max_prefill, peaks())
+    # what a step of single tokens reads of a cached one
+    read_per_token = model.cache_bytes_per_token(args.cache_bits // 8, args.page, expanded=False)
+    roofline = roofline_of(fg.step_log[log0:], cfg, model.weight_bytes(), read_per_token, gen_args.max_prefill, peaks())
     n_prompt = sum(len(p) for p, _ in reqs)
     line = {
         "impl": "ours", "workload": f"llama-{args.shape} shape, continuous batching", "requests": len(reqs),

@@ -42,3 +42,25 @@ def test_the_budget_holds_the_scales_of_an_8_bit_cache(tmp_path, page):
     expect = (int(0.103e9) - fg.model.weight_bytes() - int(0.1e9)) // per_token
     assert fg.max_seq == -(-expect // page) * page and expect > page
     fg.destroy()
+
+
+def test_what_a_step_of_single_tokens_reads(tmp_path, monkeypatch, capsys):
+    """The serving benchmark's share of the memory rate counts codes and scales of a cached token, not the pool of portions."""
+    import json
+    import sys
+    from fastgen_b200.engine import Model
+    from fastgen_b200.tools import serve_bench
+    model = Model.load(_folder(tmp_path), torch.bfloat16, DEV)
+    codes = 2 * 2 * 2 * 64  # layers, keys and values, heads of 64
+    assert model.cache_bytes_per_token(1, 64, expanded=False) == codes + 1  # 8 scales of 4 bytes a page of 64, rounded up
+    assert model.cache_bytes_per_token(1, 64) == codes + 1 + 2 * 2 * 2 * 64
+    assert model.cache_bytes_per_token(2, 64, expanded=False) == 2 * codes == model.cache_bytes_per_token(2)
+    got = []
+    plain = serve_bench.roofline_of
+    monkeypatch.setattr(serve_bench, "roofline_of", lambda log, cfg, weights, per_token, *rest: got.append(per_token) or plain(log, cfg, weights, per_token, *rest))
+    monkeypatch.setattr(sys, "argv", ["serve_bench", "--shape", "1b", "--layers", "2", "--requests", "2", "--cache-bits", "8", "--arrive-over", "0"])
+    assert serve_bench.main() == 0
+    shape = serve_bench.SHAPES["1b"]
+    heads, size = shape["num_key_value_heads"], shape["head_dim"]
+    assert got == [2 * 2 * heads * size + -(-2 * 2 * heads * 4 // 64)]
+    assert json.loads(capsys.readouterr().out.strip().splitlines()[-1])["errors"] == 0
