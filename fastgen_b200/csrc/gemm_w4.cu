@@ -15,11 +15,12 @@
 //    blocks an SM do not hide all of one another's waits.
 //  * In a chunk a lane takes 32 neighbouring columns (one 16-byte piece a row).  Groups of 32 and 64 columns must not meet in
 //    one instruction: there the four lanes of a row take a word each of the same 32 columns, four pieces of four bytes.
-#include "skinny_product.cuh"
+#include "gemm_w4.cuh"
 
 namespace {
 
 using namespace fg_skinny;
+using namespace fg_w4;
 
 constexpr int KCHUNK = 128;  // columns a warp takes at a time
 constexpr int TOKENS = 8;
@@ -28,15 +29,6 @@ constexpr int MAX_SHARE = 4;  // blocks of a cluster that split K
 __device__ __forceinline__ void cp_async_4(void* dst, const void* src, bool pred) {
   const int bytes = pred ? 4 : 0;
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
-}
-
-// the columns 2 i and 2 i + 1 of a word's eight, as bfloat16
-__device__ __forceinline__ uint32_t weights_of(uint32_t w, int i) {
-  uint32_t v;
-  asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;\n" : "=r"(v) : "r"(w >> (4 * i)));  // (a & b) | c
-  const uint32_t shift = 0x43084308u;  // 136
-  const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&shift));
-  return *reinterpret_cast<const uint32_t*>(&d);
 }
 
 // RT tiles of 16 rows a block; G columns a group
@@ -49,23 +41,6 @@ struct Plan4 {
   static constexpr size_t SUMS = (size_t)WARPS * RT * ROWS * TOKENS * 4;
   static constexpr size_t SMEM = RING + SUMS;
   static constexpr int BLOCKS = SMEM <= 75 * 1024 ? 3 : 2;  // an SM
-};
-
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-}
-__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
-  uint32_t remote;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(remote) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(remote) : "memory");
-  return v;
-}
-
-struct Epilogue4 {
-  const __nv_bfloat16* bias;  // [N] or null
-  int act;                    // ACT_*; with `gated`: 1 for a relu gate
-  bool gated;                 // rows are gate and up in blocks of 8: y[M, N / 2]
 };
 
 template <typename P, typename TO>
@@ -332,8 +307,6 @@ extern "C" int fg_w4_dense(const void* w, const void* scales, int group, void* o
   FG_CHECK_LAUNCH("fg_w4_dense");
   return 0;
 }
-
-extern "C" int fg_gemm_w4_max_m() { return TOKENS; }
 
 // x: [M, K] bf16 (row stride ldx); w: codes [N, K / 8] words (see above); scales: bf16 [N, K / group]; y: [M, N] bf16 or float32,
 // or with `gated` [M, N / 2] bf16: silu (relu with act 1) of the gate rows times the up rows, which lie in blocks of 8 in

@@ -17,12 +17,13 @@
 // 4,096 takes 25 us with 16 tokens, 30 with 64 (reading the codes 9.3, the products with 64 tokens 9.0), 57 with 128.
 #include <type_traits>
 
-#include "skinny_product.cuh"
+#include "gemm_w4.cuh"
 #include "tc5_primitives.cuh"
 #include "tensor_map.cuh"
 
 namespace {
 using namespace fg_tc5;
+using namespace fg_w4;
 
 constexpr int ROWS4 = 128;   // rows of W a tile
 constexpr int KC = 128;      // columns of a chunk
@@ -82,37 +83,11 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
   if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
-// the columns 2 i and 2 i + 1 of a word's eight, as bfloat16 (see gemm_w4.cu)
-__device__ __forceinline__ uint32_t weights_of(uint32_t w, int i) {
-  uint32_t v;
-  asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;\n" : "=r"(v) : "r"(w >> (4 * i)));
-  const uint32_t shift = 0x43084308u;  // 136
-  const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&shift));
-  return *reinterpret_cast<const uint32_t*>(&d);
-}
-
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-}
-__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
-  uint32_t remote;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(remote) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(remote) : "memory");
-  return v;
-}
-
-struct Epilogue4 {
-  const __nv_bfloat16* bias;  // [N] or null
-  int act;                    // ACT_*; with `gated`: 1 for a relu gate
-  int gated;                  // rows are gate and up in blocks of 8: y[M, N / 2]
-};
-
 // one element of the result from its sum; called by whole warps, a lane a row of W (32 neighbouring ones)
 template <typename TO>
 __device__ __forceinline__ void store_sum(float v, int m, int n, bool ok, int N, TO* y, int ldy, const Epilogue4& epi, float bias) {
@@ -431,11 +406,10 @@ int share_of(int M, int N, int K) {
 }
 
 template <int G, typename TO>
-int choose(const void* x, int ldx, const void* w, const void* scales, void* y, int ldy, int M, int N, int K, int share,
+int choose(const void* x, int ldx, const void* w, const void* scales, void* y, int ldy, int M, int N, int K,
            const Epilogue4& epi, int* status, cudaStream_t stream) {
 #define FG_W4(T)                                                                                                       \
-  return launch<Shape4<T, G>, TO>(x, ldx, w, scales, y, ldy, M, N, K, share > 0 ? share : share_of<Shape4<T, G>>(M, N, K), epi, \
-                                  status, stream)
+  return launch<Shape4<T, G>, TO>(x, ldx, w, scales, y, ldy, M, N, K, share_of<Shape4<T, G>>(M, N, K), epi, status, stream)
   if (M <= 16) FG_W4(16);
   if (M <= 32) FG_W4(32);
   if (M <= 64 || G == 32) FG_W4(64);
@@ -445,18 +419,18 @@ int choose(const void* x, int ldx, const void* w, const void* scales, void* y, i
 }
 
 template <typename TO>
-int by_group(int group, const void* x, int ldx, const void* w, const void* scales, void* y, int ldy, int M, int N, int K, int share,
+int by_group(int group, const void* x, int ldx, const void* w, const void* scales, void* y, int ldy, int M, int N, int K,
              const Epilogue4& epi, int* status, cudaStream_t stream) {
-  if (group == 128) return choose<128, TO>(x, ldx, w, scales, y, ldy, M, N, K, share, epi, status, stream);
-  if (group == 64) return choose<64, TO>(x, ldx, w, scales, y, ldy, M, N, K, share, epi, status, stream);
-  return choose<32, TO>(x, ldx, w, scales, y, ldy, M, N, K, share, epi, status, stream);
+  if (group == 128) return choose<128, TO>(x, ldx, w, scales, y, ldy, M, N, K, epi, status, stream);
+  if (group == 64) return choose<64, TO>(x, ldx, w, scales, y, ldy, M, N, K, epi, status, stream);
+  return choose<32, TO>(x, ldx, w, scales, y, ldy, M, N, K, epi, status, stream);
 }
 
 }  // namespace
 
-// Arguments as of fg_gemm_w4, any M.  share: blocks of a cluster a tile (1, 2, 4, 8), or 0 for the rule's choice.
+// Arguments as of fg_gemm_w4, any M.
 extern "C" int fg_gemm_w4_tc5(const void* x, int ldx, const void* w, const void* scales, int group, void* y, int ldy,
-                              int out_dtype, int M, int N, int K, const void* bias, int act, int gated, int share, int* status,
+                              int out_dtype, int M, int N, int K, const void* bias, int act, int gated, int* status,
                               cudaStream_t stream) {
   if (M == 0 || N == 0) return 0;
   FG_CHECK_ARG(group == 32 || group == 64 || group == 128, "fg_gemm_w4_tc5: groups of %d columns are not supported (32, 64, 128)",
@@ -466,13 +440,12 @@ extern "C" int fg_gemm_w4_tc5(const void* x, int ldx, const void* w, const void*
   FG_CHECK_ARG((((uintptr_t)x | (uintptr_t)w) & 15) == 0, "fg_gemm_w4_tc5: x and the codes must be 16-byte aligned");
   FG_CHECK_ARG(!gated || (N % 16 == 0 && bias == nullptr && out_dtype == FG_BF16), "fg_gemm_w4_tc5: a gated product of %d rows", N);
   FG_CHECK_ARG(act >= fg_skinny::ACT_NONE && act <= fg_skinny::ACT_RELU2, "fg_gemm_w4_tc5: unknown activation %d", act);
-  FG_CHECK_ARG(share == 0 || share == 1 || share == 2 || share == 4 || share == 8, "fg_gemm_w4_tc5: clusters of %d blocks", share);
-  const Epilogue4 epi{(const __nv_bfloat16*)bias, act, gated};
+  const Epilogue4 epi{(const __nv_bfloat16*)bias, act, gated != 0};
   int rc;
   if (out_dtype == FG_BF16)
-    rc = by_group<__nv_bfloat16>(group, x, ldx, w, scales, y, ldy, M, N, K, share, epi, status, stream);
+    rc = by_group<__nv_bfloat16>(group, x, ldx, w, scales, y, ldy, M, N, K, epi, status, stream);
   else if (out_dtype == FG_F32)
-    rc = by_group<float>(group, x, ldx, w, scales, y, ldy, M, N, K, share, epi, status, stream);
+    rc = by_group<float>(group, x, ldx, w, scales, y, ldy, M, N, K, epi, status, stream);
   else
     FG_CHECK_ARG(false, "fg_gemm_w4_tc5: bad output dtype %d", out_dtype);
   if (rc) return rc;

@@ -11,8 +11,6 @@
 #endif
 static_assert(FG_HEAD_DIM == 64 || FG_HEAD_DIM == 128 || FG_HEAD_DIM == 256, "head sizes 64, 128 and 256");
 
-extern "C" int fg_kv8_head_dim() { return FG_HEAD_DIM; }
-
 static int check_pages(const char* name, const void* k_pages, const void* v_pages, const float* k_scales,
                        const float* v_scales, int page_size, int n_pages, int n_kv_heads, int head_dim) {
   FG_CHECK_ARG(head_dim == FG_HEAD_DIM, "%s: library built for head size %d, got %d", name, FG_HEAD_DIM, head_dim);
@@ -100,7 +98,7 @@ extern "C" int fg_kv8_decode_scratch_floats() {
   using namespace fg_kv8;
   return decode_blocks_per_sm<FG_HEAD_DIM>() * fg_sm_count() * 2 * MAX_COLUMNS * run_stride<FG_HEAD_DIM>();
 }
-extern "C" int fg_kv8_decode_counters(int n_seqs, int n_heads, int n_kv_heads) {
+static int decode_counters(int n_seqs, int n_heads, int n_kv_heads) {
   const int group = n_heads / n_kv_heads;
   return n_seqs * n_kv_heads * ((group + fg_kv8::MAX_COLUMNS - 1) / fg_kv8::MAX_COLUMNS);
 }
@@ -120,7 +118,7 @@ extern "C" int fg_kv8_attention_decode(const void* q, int q_stride, void* out, i
                "fg_kv8_attention_decode: %d heads over %d kv heads, %d sequences (at most %d)", n_heads, n_kv_heads, n_seqs,
                DECODE_MAX_SEQS);
   FG_CHECK_ARG(scratch != nullptr && scratch_floats >= fg_kv8_decode_scratch_floats() && counters != nullptr &&
-                   n_counters >= fg_kv8_decode_counters(n_seqs, n_heads, n_kv_heads) && ((uintptr_t)scratch & 15) == 0,
+                   n_counters >= decode_counters(n_seqs, n_heads, n_kv_heads) && ((uintptr_t)scratch & 15) == 0,
                "fg_kv8_attention_decode: scratch of %d floats, %d counters are too few", scratch_floats, n_counters);
   FG_CHECK_ARG(q_stride % 8 == 0 && out_stride % 2 == 0, "fg_kv8_attention_decode: row strides %d and %d", q_stride, out_stride);
   const int group = n_heads / n_kv_heads;

@@ -26,7 +26,6 @@ SIGNATURES = {
     "fg_kv8_attention_decode": [_P, _I, _P, _I, _P, _P, _I, _P, _P, _P, _I, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _F, _F, _P,
                                 _I, _P, _I, _P, _P, _P, _P],
     "fg_kv8_decode_scratch_floats": [],
-    "fg_kv8_decode_counters": [_I, _I, _I],
 }
 _libraries = {}
 _capturing = torch.cuda.is_current_stream_capturing

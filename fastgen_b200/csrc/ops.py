@@ -94,7 +94,7 @@ _CORE_SIGNATURES = {
                                 _I, _I, _P, _P],
     "fg_gemm_w4": [_P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _P, _I, _I, _P],
     "fg_w4_dense": [_P, _P, _I, _P, _I, _I, _P],
-    "fg_gemm_w4_tc5": [_P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _P, _I, _I, _I, _P, _P],
+    "fg_gemm_w4_tc5": [_P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _P, _I, _I, _P, _P],
     "fg_sample": [_P, _I, _I, _I, _P, _F, c_ulonglong, _P, _P, _P, _P, _P, _P, _P],
     "fg_selftest_wait_timeout": [_I, _P, _P, _P],
     "fg_sample_uniform": [c_ulonglong, _P, _P, _P, _I, _P],
@@ -1148,7 +1148,7 @@ class Ops(Kv8Ops):
         else:
             _check(self.lib, self.lib.fg_gemm_w4_tc5(
                 at, ldx, w.packed.data_ptr(), w.scales.data_ptr(), w.group, out.data_ptr(), out.stride(0), _code(out.dtype),
-                m, n, k, _ptr(bias), code, gated, 0, self.status.data_ptr(), _stream()))
+                m, n, k, _ptr(bias), code, gated, self.status.data_ptr(), _stream()))
         return out
 
     def _skinny_ok(self, x: torch.Tensor, w: torch.Tensor, k: int) -> bool:
