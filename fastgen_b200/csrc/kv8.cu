@@ -51,7 +51,9 @@ extern "C" int fg_kv8_write(const void* q, int q_stride, void* q_out, const void
                   qn_w, kn_w, rstd_heads, magnitude, rot_pairs);
     return 0;
   };
-  // few tokens: a warp a token
+  // Few tokens: a warp a token.  us by that and by four tokens a warp (32 / 8 heads of 128, pages of 64): one prompt of 256 tokens 9.4
+  // and 8.6, of 512 9.6 and 9.9, of 1,024 11.6 and 10.5, two of 1,024 16.9 and 14.1; 500 single tokens 7.1 and 11.9, 1,000 10.0 and 12.0.
+  // (Pages of 16, where a stretch holds four runs, want the first: 512 tokens 9.2 and 26.3, 1,024 16.6 and 27.9.)
   const int rc = n_tokens <= 512 ? launch(vec ? kv8_write_kernel<FG_HEAD_DIM, true, 1> : kv8_write_kernel<FG_HEAD_DIM, false, 1>, 1)
                                  : launch(vec ? kv8_write_kernel<FG_HEAD_DIM, true, 4> : kv8_write_kernel<FG_HEAD_DIM, false, 4>, 4);
   if (rc) return rc;

@@ -56,6 +56,7 @@ constexpr float WEIGHT_UNIT = 1.f / (1 << WEIGHT_SHIFT);
 constexpr int SCALES_NEAR = 64;      // exponents of values' scales this close take the short way to a denominator
 constexpr int NO_PAGE = -1000;       // in an exponent's place
 
+// As many slots as an SM's blocks have room for.  (Fewer, 4 / 3 / 2, or eight of the smallest: every case within 2 %.)
 template <int HD>
 __host__ __device__ constexpr int decode_slots() { return HD == 64 ? 6 : HD == 128 ? 4 : 3; }
 template <int HD>

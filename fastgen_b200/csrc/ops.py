@@ -135,7 +135,11 @@ _ATTN_SIGNATURES = {
 
 SKINNY_MAX_M = int(os.environ.get("FG_SKINNY_MAX_M", "8"))      # most tokens the weight-streaming product is used for (it takes up to 32)
 W4_MAX_M = 8         # most tokens of the product that streams 4-bit weights; more go to tcgen05
-W4_DENSE_M = 256     # tokens from which 4-bit weights are expanded for the product of 16-bit ones
+# Tokens from which 4-bit weights are expanded for the product of 16-bit ones.  us by that and by the product of its own (which unpacks
+# the weights anew for every 64 or 128 tokens), groups of 128: 28,672 x 4,096 110 and 103 at 192 tokens, 111 and 112 at 256, 126 and
+# 142 at 384; 4,096 x 14,336 58 and 46 at 256, 68 and 78 at 384; 6,144 x 4,096 18 and 21 at 128, 21 and 29 at 256.  (Groups of
+# 32: 28,672 x 4,096 112 and 206 at 256.)
+W4_DENSE_M = 256
 SIMT_ROWS = 16       # query rows per block of the float32 attention kernel
 F32_PROMPT_ROWS = 64  # ... of the float32 kernel of larger prompts
 PREFILL_ROWS = 64    # ... of the bfloat16 prompt kernel
@@ -1055,7 +1059,7 @@ class Ops(Kv8Ops):
         ``bias`` [N] of the compute dtype and ``act`` (a key of ``ACTIVATIONS``) are optional.  The
         bias is added to the float32 sums; the activation sees the rounded result.  ``w`` may be a
         :class:`~fastgen_b200.weights.Weight4` (bfloat16 only): its whole numbers enter the product as they are and a
-        group's float32 sums are multiplied by its scale."""
+        group's float32 sums are multiplied by its scale; from ``W4_DENSE_M`` tokens on each weight is rounded to bfloat16 first."""
         if isinstance(w, Weight4):
             return self._linear4(x, w, out, out_dtype, bias, act)
         m, k = x.shape

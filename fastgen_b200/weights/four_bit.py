@@ -1,8 +1,8 @@
 """Matrices of 4-bit weights with a scale for each group of columns of a row.
 
 ``W[n, k] = (code[n, k] - 8) * scale[n, k // group]``: codes 0..15, groups of 32, 64 or 128 columns, scales in
-bfloat16.  :meth:`Weight4.quantize` makes one from a matrix; a checkpoint's own codes and scales go through the
-constructor.  :meth:`fastgen_b200.csrc.ops.Ops.linear` multiplies by it as by an ordinary matrix.
+bfloat16.  :meth:`Weight4.quantize` makes one from a matrix, as a model's projections become 4-bit weights when they are
+bound; codes and scales that a program has already go through the constructor.  :meth:`fastgen_b200.csrc.ops.Ops.linear` multiplies by it as by an ordinary matrix.
 """
 
 from __future__ import annotations
