@@ -15,6 +15,7 @@
 //    blocks an SM do not hide all of one another's waits.
 //  * In a chunk a lane takes 32 neighbouring columns (one 16-byte piece a row).  Groups of 32 and 64 columns must not meet in
 //    one instruction: there the four lanes of a row take a word each of the same 32 columns, four pieces of four bytes.
+//    (28,672 x 4,096, one token: groups of 128 20 us, 64 41, 32 55; weights in 16 bits 37.)
 #include "gemm_w4.cuh"
 
 namespace {

@@ -126,7 +126,7 @@ def _near_borders(size, page, place, magnitude, pairs, seed, factors=None):
 
 @pytest.mark.parametrize("size,page", [(64, 16), (128, 64), (256, 256)])
 @pytest.mark.parametrize("way", ["single", "behind", "run", "run behind"])
-@pytest.mark.parametrize("option", ["keys", "values", "norm", "magnitude"])
+@pytest.mark.parametrize("option", ["keys", "values", "norm", "norm a head", "magnitude"])
 def test_scales_next_to_a_border(ops, size, page, way, option):
     """A page whose largest turned number lies within 2^-22 of 448 * 2^e, on either side of it: the smallest 2^e at which 448
     reaches that number's 64-bit value.  (Float32 sees one in ten of them on the wrong side.)"""
@@ -135,7 +135,7 @@ def test_scales_next_to_a_border(ops, size, page, way, option):
     first = 2 if "behind" in way else 0  # tokens of the page that are cached before
     magnitude, pairs = (1.25, size // 4) if option == "magnitude" else (1.0, 0)
     g = torch.Generator().manual_seed(size)
-    weights = (0.5 + torch.rand(size, generator=g)).to(DEV) if option == "norm" else None
+    weights = (0.5 + torch.rand(size, generator=g)).to(DEV) if option.startswith("norm") else None
     freqs, (pair, pos, a, b, rstd, big) = _near_borders(size, page, place, magnitude, pairs, size + len(way), weights)
     n = pair.numel()
     assert n > 100
@@ -158,9 +158,14 @@ def test_scales_next_to_a_border(ops, size, page, way, option):
                            None, memory, 1, 1, size)
     at = (start + begin + torch.arange(tokens, device=DEV)).flatten().to(torch.int32)
     req = each.repeat_interleave(tokens).to(torch.int32)
-    norm = (rstd.repeat_interleave(tokens)[:, None].expand(-1, 2).contiguous(), weights, weights) if option == "norm" else None
+    heads, norm = 1, None
+    if option.startswith("norm"):
+        heads = 3 if option == "norm a head" else 1
+        factors = torch.full((n * tokens, heads + 1), 7.0, device=DEV)  # (the last column is the keys')
+        factors[:, -1] = rstd.repeat_interleave(tokens)
+        norm = factors, weights.repeat(heads), weights
     k, v = (nothing, rows) if option == "values" else (rows, nothing)
-    ops.rope_kv8_write(nothing, k, v, at, req, freqs, memory, 1, 1, size, v_freqs=freqs if option == "values" else None, qk_norm=norm,
+    ops.rope_kv8_write(nothing.repeat(1, heads), k, v, at, req, freqs, memory, heads, 1, size, v_freqs=freqs if option == "values" else None, qk_norm=norm,
                        magnitude=magnitude, rot_pairs=pairs)
     ops.check_status()
     scales = (memory.v_scales if option == "values" else memory.k_scales)[table[:, 0].long(), 0].double()
