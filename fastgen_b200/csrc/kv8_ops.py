@@ -72,6 +72,7 @@ class Kv8Ops:
         # (head size, stream) -> partials and counters of the single-token attention over a cache in 8 bits; the stream of
         # captured calls is None
         self._kv8_buffers = {}
+        self._growing = threading.Lock()
         self._kv8_retired = []
 
     def _clear_kv8(self) -> None:
@@ -225,17 +226,18 @@ class Kv8Ops:
         got = self._kv8_buffers.get((head_dim, stream))
         if got is None or got[1].numel() < counters:
             n = max(1024, 1 << (counters - 1).bit_length())
-            for key in ((head_dim, stream), (head_dim, None)):
-                old = self._kv8_buffers.get(key)
-                if old is not None and old[1].numel() >= n:
-                    continue
-                scratch = old[0] if old is not None else torch.empty(lib.fg_kv8_decode_scratch_floats(), dtype=torch.float32,
-                                                                     device=self.device)
-                if old is not None:
-                    self._kv8_retired.append(old[1])
-                self._kv8_buffers[key] = (scratch, torch.zeros(n, dtype=torch.int32, device=self.device))
-            torch.cuda.current_stream(self.device).synchronize()  # graphs are replayed on any stream
-            got = self._kv8_buffers[head_dim, stream]
+            with self._growing:
+                for key in ((head_dim, stream), (head_dim, None)):
+                    old = self._kv8_buffers.get(key)
+                    if old is not None and old[1].numel() >= n:
+                        continue
+                    scratch = old[0] if old is not None else torch.empty(lib.fg_kv8_decode_scratch_floats(), dtype=torch.float32,
+                                                                         device=self.device)
+                    if old is not None:
+                        self._kv8_retired.append(old[1])
+                    self._kv8_buffers[key] = (scratch, torch.zeros(n, dtype=torch.int32, device=self.device))
+                torch.cuda.current_stream(self.device).synchronize()  # graphs are replayed on any stream
+                got = self._kv8_buffers[head_dim, stream]
         return got
 
     def _attention_kv8(self, q, out, memory, ctx, n_heads, n_kv_heads, head_dim, window, scale, out_freqs, keep_first,
